@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libanchor_attn_b200.so")
 
 AA_OK = 0
 AA_BF16 = 0
+AA_E4M3 = 1
 
 EXPORTS = [
     "aa_workspace_bytes", "aa_workspace_layout", "aa_id_row_offset", "aa_forward",
@@ -20,6 +21,8 @@ EXPORTS = [
     "aa_selftest_wait_timeout", "aa_block_sparse_workspace_bytes", "aa_block_sparse_attend",
     "aa_block_sparse_check_status", "aa_validate_lists", "aa_step2_stripes_static_check_status",
     "aa_peer_barrier", "aa_dense_causal_attend", "aa_rope_dispatch",
+    "aa_paged_append", "aa_paged_attend", "aa_paged_attend_workspace_bytes", "aa_page_select",
+    "aa_paged_check_status",
 ]
 MAX_PEERS = 8
 STATIC_SCRATCH_BYTES = 8 << 20
@@ -110,6 +113,38 @@ class AAPeerBarrier(ctypes.Structure):
                 ("timeout_ms", ctypes.c_uint32), ("flags", ctypes.c_void_p * MAX_PEERS), ("status", ctypes.c_void_p)]
 
 
+class AAPagedCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages")] + [
+        (f"{t}_stride_{a}", ctypes.c_int64) for t in "kv" for a in ("page", "head", "row")] + [
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p), ("status", ctypes.c_void_p)] + [
+        (n, ctypes.c_int32) for n in ("pages", "page_size", "table_width", "Hkv", "D", "cache_dtype", "B")]
+
+
+class AAPagedAppend(ctypes.Structure):
+    _fields_ = [("cache", AAPagedCache)] + [
+        (n, ctypes.c_void_p) for n in ("key", "value", "query", "query_out", "key_out")] + [
+        (f"{t}_stride_{a}", ctypes.c_int64) for t in ("key", "value", "query", "query_out", "key_out") for a in "th"] + [
+        (n, ctypes.c_void_p) for n in ("cu_seqlens", "cos", "sin", "key_codes", "key_code_scales")] + [
+        (n, ctypes.c_int32) for n in ("rope_rows", "T", "H", "reserved")]
+
+
+class AAPagedAttend(ctypes.Structure):
+    _fields_ = [("cache", AAPagedCache), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p)] + [
+        (f"{t}_stride_{a}", ctypes.c_int64) for t in "qo" for a in "bnh"] + [
+        (n, ctypes.c_void_p) for n in ("pages", "page_counts", "workspace")] + [
+        ("workspace_bytes", ctypes.c_size_t), ("sm_scale", ctypes.c_double)] + [
+        (n, ctypes.c_int32) for n in ("list_width", "Nq", "H", "reserved")]
+
+
+class AAPageSelect(ctypes.Structure):
+    _fields_ = [("cache", AAPagedCache), ("q", ctypes.c_void_p)] + [
+        (f"q_stride_{a}", ctypes.c_int64) for a in "bnh"] + [
+        (n, ctypes.c_void_p) for n in ("key_codes", "key_code_scales", "out", "counts")] + [
+        (n, ctypes.c_int32) for n in ("Nq", "H", "top", "keep_first", "keep_last", "reserved")]
+
+
 _lib = None
 
 
@@ -150,6 +185,14 @@ def load():
     for name in ("aa_block_sparse_attend", "aa_block_sparse_check_status"):
         getattr(lib, name).argtypes = [PB, ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
+    for name, struct in (("aa_paged_append", AAPagedAppend), ("aa_paged_attend", AAPagedAttend),
+                         ("aa_page_select", AAPageSelect)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.aa_paged_attend_workspace_bytes.argtypes = [ctypes.POINTER(AAPagedAttend), ctypes.POINTER(ctypes.c_size_t)]
+    lib.aa_paged_attend_workspace_bytes.restype = ctypes.c_int
+    lib.aa_paged_check_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    lib.aa_paged_check_status.restype = ctypes.c_int
     lib.aa_total_selected.argtypes = [P, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]
     lib.aa_forward_launches.argtypes = [P]
     lib.aa_forward_launches.restype = ctypes.c_int

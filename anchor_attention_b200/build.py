@@ -9,7 +9,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libanchor_attn_b200.so")
-SOURCES = ["anchor_abi.cu"]
+SOURCES = ["anchor_abi.cu", "paged_abi.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--expt-relaxed-constexpr", "-shared", "-Xcompiler", "-fPIC", "-cudart", "shared",

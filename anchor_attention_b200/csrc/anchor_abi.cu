@@ -28,6 +28,15 @@ int cuda_fail(cudaError_t e, const char* what) {
     return AA_ERR_CUDA;
 }
 
+}  // namespace
+
+// the other source files of the library record their CUDA errors here
+namespace aa {
+int record_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+}  // namespace aa
+
+namespace {
+
 size_t align_up(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }
 
 int check_shape(const aa_params_t* p) {
@@ -1017,6 +1026,10 @@ const char* aa_strerror(int code) {
         case AA_ERR_TOO_LARGE: return "problem too large for this entry point";
         case AA_ERR_UNSORTED: return "a block list is not in ascending order";
         case AA_ERR_BAD_LIST: return "an id list in the workspace is malformed (count or id out of range, or not ascending)";
+        case AA_ERR_PAGE_SIZE: return "page_size must be a power of two from 16 to 256, pool and block table not empty";
+        case AA_ERR_NEW_TOKENS: return "too many new tokens (or new tokens times query heads per KV head) for a decode call";
+        case AA_ERR_BAD_PAGE: return "a page number lies outside the pool, or a page-list entry outside its sequence";
+        case AA_ERR_TOO_LONG: return "a sequence is longer than its row of the block table, or than the rotary tables";
         default: return "unknown error";
     }
 }

@@ -1,0 +1,332 @@
+// C ABI of the paged key-value cache: argument checks and launches.  Declarations are in
+// include/anchor_attn_b200.h.
+#include "../../include/anchor_attn_b200.h"
+
+#include <math.h>
+
+#include "page_select.cuh"
+#include "paged_append.cuh"
+#include "paged_attend.cuh"
+
+namespace aa {
+int record_cuda_error(cudaError_t e, const char* what);      // anchor_abi.cu
+}
+
+namespace {
+
+using aa::record_cuda_error;
+
+struct Device {
+    int id = -1, sms = 0;
+};
+
+// The current device and its SM count; raises the shared-memory limit of the kernels on a thread's first call
+// for a device.
+template <typename F>
+int current_device(Device& known, F&& configure) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return record_cuda_error(e, "cudaGetDevice");
+    if (known.id != dev) {
+        e = cudaDeviceGetAttribute(&known.sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return record_cuda_error(e, "cudaDeviceGetAttribute(SM count)");
+        e = configure();
+        if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(paged cache)");
+        known.id = dev;
+    }
+    return AA_OK;
+}
+
+bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+bool bad_stride(int64_t s, int elements = 8) { return s % elements != 0; }
+
+// table, lengths and shapes; log2 of the page size
+int check_table(const aa_paged_cache_t& c, int* log2_page) {
+    if (c.B <= 0 || c.Hkv <= 0) return AA_ERR_SHAPE;
+    if (c.D != 128) return AA_ERR_HEAD_DIM;
+    if (c.pages <= 0 || c.table_width <= 0 || c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)))
+        return AA_ERR_PAGE_SIZE;
+    if (!c.block_table || !c.seq_lens || !c.status) return AA_ERR_NULL;
+    if ((int64_t)c.table_width * c.page_size > (int64_t)1 << 30 || (int64_t)c.B * c.Hkv > 1 << 24) return AA_ERR_TOO_LARGE;
+    *log2_page = 31 - __builtin_clz((unsigned)c.page_size);
+    return AA_OK;
+}
+
+int check_pools(const aa_paged_cache_t& c) {
+    if (!c.k_pages || !c.v_pages) return AA_ERR_NULL;
+    if (c.cache_dtype != AA_BF16 && c.cache_dtype != AA_E4M3) return AA_ERR_DTYPE;
+    if (c.cache_dtype == AA_E4M3 && (!c.k_scale || !c.v_scale)) return AA_ERR_NULL;
+    const int unit = c.cache_dtype == AA_E4M3 ? 16 : 8;
+    for (int64_t s : {c.k_stride_page, c.k_stride_head, c.k_stride_row, c.v_stride_page, c.v_stride_head, c.v_stride_row})
+        if (bad_stride(s, unit)) return AA_ERR_STRIDE;
+    if (misaligned(c.k_pages) || misaligned(c.v_pages)) return AA_ERR_STRIDE;
+    return AA_OK;
+}
+
+aa::paged::Cache view(const aa_paged_cache_t& c, int log2_page) {
+    const int64_t size = c.cache_dtype == AA_E4M3 ? 1 : 2;
+    aa::paged::Cache v;
+    v.k = {static_cast<uint8_t*>(c.k_pages), c.k_stride_page * size, c.k_stride_head * size, c.k_stride_row * size};
+    v.v = {static_cast<uint8_t*>(c.v_pages), c.v_stride_page * size, c.v_stride_head * size, c.v_stride_row * size};
+    v.k_scale = c.k_scale;
+    v.v_scale = c.v_scale;
+    v.table = c.block_table;
+    v.table_stride = c.table_stride;
+    v.table_width = c.table_width;
+    v.pages = c.pages;
+    v.log2_page = log2_page;
+    v.seq_lens = c.seq_lens;
+    v.status = c.status;
+    return v;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// ---- attention: how a call is cut up
+struct AttendPlan {
+    int log2_page, rows, row_tiles, tiles8;       // tiles8: tiles of 8 rows one CTA holds (1 .. 4)
+    int ctas;
+    bool split;                                   // whether an entry can be cut at all
+    size_t o_off, ml_off, cut_off, bytes;
+};
+
+template <bool FP8, int NT>
+cudaError_t allow_smem() {
+    return cudaFuncSetAttribute(aa::paged::paged_attend_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                aa::paged::kSmemBytes);
+}
+
+int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
+    if (!a) return AA_ERR_NULL;
+    const aa_paged_cache_t& c = a->cache;
+    int rc = check_table(c, &pl.log2_page);
+    if (rc) return rc;
+    if (a->H <= 0 || a->H % c.Hkv || a->Nq <= 0) return AA_ERR_SHAPE;
+    if (a->Nq > aa::paged::kMaxNew) return AA_ERR_NEW_TOKENS;
+    if (a->pages && (a->list_width <= 0 || !a->page_counts)) return a->page_counts ? AA_ERR_SHAPE : AA_ERR_NULL;
+    if (a->pages && (int64_t)a->list_width * c.page_size > (int64_t)1 << 30) return AA_ERR_TOO_LARGE;
+    static thread_local Device dev;
+    rc = current_device(dev, [] {
+        for (cudaError_t e : {allow_smem<false, 1>(), allow_smem<false, 2>(), allow_smem<false, 3>(), allow_smem<false, 4>(),
+                              allow_smem<true, 1>(), allow_smem<true, 2>(), allow_smem<true, 3>(), allow_smem<true, 4>()})
+            if (e != cudaSuccess) return e;
+        return cudaSuccess;
+    });
+    if (rc) return rc;
+    if ((int64_t)a->Nq * (a->H / c.Hkv) > 1 << 16) return AA_ERR_NEW_TOKENS;
+    pl.rows = a->Nq * (a->H / c.Hkv);
+    // rows in as few tiles of up to 32 as there can be (each reads the cache), the tiles alike
+    pl.row_tiles = (int)ceil_div(pl.rows, 32);
+    pl.tiles8 = (int)ceil_div(ceil_div(pl.rows, pl.row_tiles), 8);
+    const int64_t entries = (int64_t)c.B * c.Hkv * pl.row_tiles;
+    const int64_t keys = (int64_t)(a->pages ? a->list_width : c.table_width) * c.page_size;
+    const int64_t units = ceil_div(keys, aa::paged::kUnitKeys);
+    if (entries * units > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
+    const int64_t most = (int64_t)dev.sms * aa::paged::kCtasPerSm;
+    pl.ctas = (int)(entries * units < most ? entries * units : most);
+    if (pl.ctas > 512) pl.ctas = 512;             // the join kernel's table of weights
+    pl.split = units > 1 && pl.ctas > 1;
+    const size_t parts = pl.split ? (size_t)pl.ctas * 2 * 8 * pl.tiles8 : 0;
+    pl.o_off = 0;
+    pl.ml_off = align256(parts * aa::kD * sizeof(float));
+    pl.cut_off = align256(pl.ml_off + parts * sizeof(float2));
+    pl.bytes = align256(pl.cut_off + pl.ctas * sizeof(int32_t));
+    return AA_OK;
+}
+
+template <bool FP8, int NT>
+int launch_attend(const aa::paged::AttendParams& p, const AttendPlan& pl, cudaStream_t st) {
+    aa::paged::paged_attend_kernel<FP8, NT><<<pl.ctas, aa::paged::kThreads, aa::paged::kSmemBytes, st>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return record_cuda_error(e, "launch paged_attend");
+    if (!pl.split) return AA_OK;
+    // the join kernel's launch overlaps the attention kernel's end; it waits on the device for its results
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pl.ctas - 1, 8 * NT < pl.rows ? 8 * NT : pl.rows);
+    cfg.blockDim = dim3(aa::paged::kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, pl.ctas, 8 * NT);
+    if (e != cudaSuccess) return record_cuda_error(e, "launch paged_join");
+    return AA_OK;
+}
+
+template <bool FP8>
+int launch_attend_rows(const aa::paged::AttendParams& p, const AttendPlan& pl, cudaStream_t st) {
+    switch (pl.tiles8) {
+        case 1: return launch_attend<FP8, 1>(p, pl, st);
+        case 2: return launch_attend<FP8, 2>(p, pl, st);
+        case 3: return launch_attend<FP8, 3>(p, pl, st);
+        default: return launch_attend<FP8, 4>(p, pl, st);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int aa_paged_check_status(uint32_t* status, void* stream) {
+    if (!status) return AA_ERR_NULL;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint32_t word = 0;
+    cudaError_t e = cudaMemcpyAsync(&word, status, sizeof(word), cudaMemcpyDeviceToHost, st);
+    if (e != cudaSuccess) return record_cuda_error(e, "cudaMemcpyAsync(status)");
+    e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return record_cuda_error(e, "cudaStreamSynchronize");
+    if (!word) return AA_OK;
+    e = cudaMemsetAsync(status, 0, sizeof(word), st);
+    if (e != cudaSuccess) return record_cuda_error(e, "cudaMemsetAsync(status)");
+    return word & aa::paged::kStatusBadPage ? AA_ERR_BAD_PAGE : AA_ERR_TOO_LONG;
+}
+
+int aa_paged_append(const aa_paged_append_t* a, void* stream) {
+    if (!a) return AA_ERR_NULL;
+    const aa_paged_cache_t& c = a->cache;
+    int log2_page = 0;
+    int rc = check_table(c, &log2_page);
+    if (rc) return rc;
+    rc = check_pools(c);
+    if (rc) return rc;
+    if (a->T <= 0 || a->H < 0 || (a->query && (a->H <= 0 || a->H % c.Hkv))) return AA_ERR_SHAPE;
+    if (!a->cu_seqlens && a->T % c.B) return AA_ERR_SHAPE;
+    if (!a->key || !a->value || (a->query && !a->query_out)) return AA_ERR_NULL;
+    if (!a->cos != !a->sin || !a->key_codes != !a->key_code_scales) return AA_ERR_NULL;
+    if (a->cos && a->rope_rows <= 0) return AA_ERR_SHAPE;
+    for (int64_t s : {a->key_stride_t, a->key_stride_h, a->value_stride_t, a->value_stride_h, a->query_stride_t, a->query_stride_h,
+                      a->query_out_stride_t, a->query_out_stride_h, a->key_out_stride_t, a->key_out_stride_h})
+        if (bad_stride(s)) return AA_ERR_STRIDE;
+    for (const void* p : {a->key, a->value, a->query, (const void*)a->query_out, (const void*)a->key_out, (const void*)a->cos,
+                          (const void*)a->sin})
+        if (misaligned(p)) return AA_ERR_STRIDE;
+    if (2 * (int64_t)c.Hkv > 65535) return AA_ERR_TOO_LARGE;
+
+    aa::paged::AppendParams p;
+    p.c = view(c, log2_page);
+    auto rows = [](const void* ptr, int64_t token, int64_t head) {
+        return aa::paged::Rows{static_cast<__nv_bfloat16*>(const_cast<void*>(ptr)), token, head};
+    };
+    p.key = rows(a->key, a->key_stride_t, a->key_stride_h);
+    p.value = rows(a->value, a->value_stride_t, a->value_stride_h);
+    p.query = rows(a->query, a->query_stride_t, a->query_stride_h);
+    p.query_out = rows(a->query_out, a->query_out_stride_t, a->query_out_stride_h);
+    p.key_out = rows(a->key_out, a->key_out_stride_t, a->key_out_stride_h);
+    p.cu = a->cu_seqlens;
+    p.cos = a->cos;
+    p.sin = a->sin;
+    p.rope_rows = a->rope_rows;
+    p.codes = a->key_codes;
+    p.code_scales = a->key_code_scales;
+    p.T = a->T;
+    p.B = c.B;
+    p.H = a->H;
+    p.Hkv = c.Hkv;
+    p.Hg = a->query ? a->H / c.Hkv : 0;
+    p.per_seq = a->cu_seqlens ? 0 : a->T / c.B;
+    // n tokens touch at most (n - 1) / page_size + 2 pages, one token one page
+    int64_t tasks;
+    if (a->cu_seqlens)
+        tasks = a->T / c.page_size + 2 * (int64_t)c.B;
+    else
+        tasks = p.per_seq == 1 ? c.B : c.B * ((p.per_seq - 1) / c.page_size + (int64_t)2);
+    if (tasks > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
+    const dim3 grid((unsigned)tasks, (unsigned)(a->query ? 2 * c.Hkv : c.Hkv));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (c.cache_dtype == AA_E4M3)
+        aa::paged::paged_append_kernel<true><<<grid, aa::paged::kAppendThreads, 0, st>>>(p);
+    else
+        aa::paged::paged_append_kernel<false><<<grid, aa::paged::kAppendThreads, 0, st>>>(p);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch paged_append");
+}
+
+int aa_paged_attend_workspace_bytes(const aa_paged_attend_t* a, size_t* bytes) {
+    if (!bytes) return AA_ERR_NULL;
+    AttendPlan pl;
+    int rc = plan_attend(a, pl);
+    if (rc) return rc;
+    *bytes = pl.bytes;
+    return AA_OK;
+}
+
+int aa_paged_attend(const aa_paged_attend_t* a, void* stream) {
+    AttendPlan pl;
+    int rc = plan_attend(a, pl);
+    if (rc) return rc;
+    const aa_paged_cache_t& c = a->cache;
+    rc = check_pools(c);
+    if (rc) return rc;
+    if (!a->q || !a->out) return AA_ERR_NULL;
+    for (int64_t s : {a->q_stride_b, a->q_stride_n, a->q_stride_h, a->o_stride_b, a->o_stride_n, a->o_stride_h})
+        if (bad_stride(s)) return AA_ERR_STRIDE;
+    if (misaligned(a->q) || misaligned(a->out)) return AA_ERR_STRIDE;
+    if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < pl.bytes) return AA_ERR_WORKSPACE;
+
+    aa::paged::AttendParams p;
+    p.c = view(c, pl.log2_page);
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.q_sb = a->q_stride_b; p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h;
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.o_sb = a->o_stride_b; p.o_sn = a->o_stride_n; p.o_sh = a->o_stride_h;
+    p.lse = a->lse;
+    p.pages = a->pages;
+    p.page_counts = a->page_counts;
+    p.list_width = a->list_width;
+    p.B = c.B; p.H = a->H; p.Hkv = c.Hkv; p.Hg = a->H / c.Hkv; p.nq = a->Nq;
+    p.rows = pl.rows;
+    p.row_tiles = pl.row_tiles;
+    const double scale = a->sm_scale != 0.0 ? a->sm_scale : 1.0 / sqrt((double)c.D);
+    p.scale_log2 = (float)(scale * 1.4426950408889634);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
+    p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
+    p.cut_entry = reinterpret_cast<int32_t*>(ws + pl.cut_off);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return c.cache_dtype == AA_E4M3 ? launch_attend_rows<true>(p, pl, st) : launch_attend_rows<false>(p, pl, st);
+}
+
+int aa_page_select(const aa_page_select_t* a, void* stream) {
+    if (!a) return AA_ERR_NULL;
+    const aa_paged_cache_t& c = a->cache;
+    int log2_page = 0;
+    int rc = check_table(c, &log2_page);
+    if (rc) return rc;
+    if (a->H <= 0 || a->H % c.Hkv || a->Nq <= 0 || a->top <= 0) return AA_ERR_SHAPE;
+    if (a->keep_first < 0 || a->keep_last < 1 || (int64_t)a->keep_first + a->keep_last > a->top) return AA_ERR_SHAPE;
+    if (a->Nq > aa::paged::kMaxNew || (int64_t)a->Nq * (a->H / c.Hkv) > aa::paged::kMaxSelectRows) return AA_ERR_NEW_TOKENS;
+    if (c.table_width > aa::paged::kMaxSelectPages) return AA_ERR_TOO_LARGE;
+    if (!a->q || !a->key_codes || !a->key_code_scales || !a->out || !a->counts) return AA_ERR_NULL;
+    for (int64_t s : {a->q_stride_b, a->q_stride_n, a->q_stride_h})
+        if (bad_stride(s)) return AA_ERR_STRIDE;
+    if (misaligned(a->q) || misaligned(a->key_codes)) return AA_ERR_STRIDE;
+    static thread_local Device dev;
+    rc = current_device(dev, [] {
+        return cudaFuncSetAttribute(aa::paged::page_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)aa::paged::select_smem_bytes(aa::paged::kMaxSelectRows, aa::paged::kMaxSelectPages));
+    });
+    if (rc) return rc;
+
+    aa::paged::SelectParams p;
+    p.c = view(c, log2_page);
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.q_sb = a->q_stride_b; p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h;
+    p.codes = a->key_codes;
+    p.code_scales = a->key_code_scales;
+    p.out = a->out;
+    p.counts = a->counts;
+    p.B = c.B; p.H = a->H; p.Hkv = c.Hkv; p.Hg = a->H / c.Hkv; p.nq = a->Nq;
+    p.rows = a->Nq * p.Hg;
+    p.top = a->top;
+    p.keep_first = a->keep_first;
+    p.keep_last = a->keep_last;
+    const size_t smem = aa::paged::select_smem_bytes(p.rows, c.table_width);
+    aa::paged::page_select_kernel<<<c.B * c.Hkv, aa::paged::kSelectThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch page_select");
+}
+
+}  // extern "C"

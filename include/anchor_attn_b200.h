@@ -38,10 +38,14 @@ enum {
     AA_ERR_DEVICE_TIMEOUT = -11,/* a bounded device-side wait gave up (status word)  */
     AA_ERR_TOO_LARGE = -12,    /* size beyond what an entry point supports           */
     AA_ERR_UNSORTED = -13,     /* a key-block list of the comparator is not ascending */
-    AA_ERR_BAD_LIST = -14      /* aa_validate_lists found a count or an id out of range  */
+    AA_ERR_BAD_LIST = -14,     /* aa_validate_lists found a count or an id out of range  */
+    AA_ERR_PAGE_SIZE = -15,    /* page_size not a power of two from 16 to 256, or an empty pool or block table */
+    AA_ERR_NEW_TOKENS = -16,   /* more new tokens (or new tokens * group) than a decode entry point takes */
+    AA_ERR_BAD_PAGE = -17,     /* a page number outside the pool, or a list entry outside its sequence (status word) */
+    AA_ERR_TOO_LONG = -18      /* a sequence beyond its block-table row or the rotary tables (status word) */
 };
 
-enum { AA_BF16 = 0 };
+enum { AA_BF16 = 0, AA_E4M3 = 1 };   /* AA_E4M3: page pools only */
 
 /*
  * Problem description.  Logical tensor shapes:
@@ -353,6 +357,117 @@ typedef struct aa_dense_causal {
     int32_t *status;
 } aa_dense_causal_t;
 int aa_dense_causal_attend(const aa_dense_causal_t *a, void *stream);
+
+/*
+ * Token generation behind a prefill: a paged key-value cache, what appends to it, what attends over it and
+ * what picks the pages of a long one.  (No counterpart in the reference, whose decode calls flash-attn on
+ * contiguous tensors, modules/llama/anchor_attention.py:101-113.)
+ *
+ * Pools: k_pages, v_pages [pages, Hkv, page_size, 128], bf16 or e4m3.  An e4m3 code of head h stands for
+ * code * k_scale[h] (v_scale[h]).  The 128 values of a row are contiguous; the other strides, in ELEMENTS, are
+ * free as long as every row starts on a 16-byte boundary (multiples of 8 for bf16, 16 for e4m3), so both
+ * [pages, Hkv, page_size, 128] and [pages, page_size, Hkv, 128] memory is accepted.  page_size is a power of two
+ * from 16 to 256.
+ * block_table int32 [B, table_width] (rows table_stride elements apart) names the pool pages of every sequence in
+ * order; entries behind a sequence's last page are not read.  seq_lens int32 [B] counts a sequence's tokens, new
+ * ones included; 0 marks padding.
+ * Device memory that is wrong is not turned into an address: a page number outside the pool is left out (nothing
+ * is written, its keys are not attended), a length beyond the table row is cut, and a bit of *status is set (1:
+ * page number, 2: length).  *status is never cleared by a launch; aa_paged_check_status reads and clears it.
+ */
+typedef struct aa_paged_cache {
+    void   *k_pages, *v_pages;
+    int64_t k_stride_page, k_stride_head, k_stride_row;
+    int64_t v_stride_page, v_stride_head, v_stride_row;
+    const float *k_scale, *v_scale;    /* [Hkv], AA_E4M3 only                          */
+    const int32_t *block_table;
+    int64_t table_stride;
+    const int32_t *seq_lens;
+    uint32_t *status;                  /* device word, zeroed by the caller once       */
+    int32_t pages, page_size, table_width;
+    int32_t Hkv, D;
+    int32_t cache_dtype;               /* AA_BF16 or AA_E4M3                           */
+    int32_t B;
+} aa_paged_cache_t;
+
+/* Reads the status word (synchronises the stream), clears it: AA_OK, AA_ERR_BAD_PAGE or AA_ERR_TOO_LONG. */
+int aa_paged_check_status(uint32_t *status, void *stream);
+
+/*
+ * Appends T new tokens: key, value [T, Hkv, 128] bf16 (strides in elements, multiples of 8).  Sequence b owns the
+ * tokens cu_seqlens[b] .. cu_seqlens[b+1] - 1 (cu_seqlens int32 [B+1]), or T / B tokens each where
+ * cu_seqlens is NULL; they take the positions seq_lens[b] - n .. seq_lens[b] - 1, and what falls on a negative
+ * position is padding and is left out, as are tokens behind cu_seqlens[B].  With cos / sin (fp32 [rope_rows, 64],
+ * contiguous) keys are rotated with the rotate-half formulation by their position's row, in 32 bits and rounded
+ * once; query [T, H, 128] likewise into query_out (NULL: no queries), rotated keys also into key_out (NULL:
+ * not wanted).  A sequence must not share a page it appends to.
+ * key_codes int8 [pages, Hkv, 128] and key_code_scales fp32 [pages, Hkv] (contiguous; both NULL: not kept): every
+ * page whose last row this call writes gets the mean of its stored keys in 8 bits, scale = max|mean| * (1 / 127)
+ * (32-bit numbers), code = rint(mean / scale); scale 0 where a key is not finite.  One launch.
+ */
+typedef struct aa_paged_append {
+    aa_paged_cache_t cache;
+    const void *key, *value, *query;
+    void *query_out, *key_out;
+    int64_t key_stride_t, key_stride_h, value_stride_t, value_stride_h;
+    int64_t query_stride_t, query_stride_h, query_out_stride_t, query_out_stride_h;
+    int64_t key_out_stride_t, key_out_stride_h;
+    const int32_t *cu_seqlens;
+    const float *cos, *sin;
+    int8_t *key_codes;
+    float  *key_code_scales;
+    int32_t rope_rows, T, H;
+    int32_t reserved;
+} aa_paged_append_t;
+int aa_paged_append(const aa_paged_append_t *a, void *stream);
+
+/*
+ * Attention of the last Nq tokens of every sequence (1 .. 16) over its cached ones: row j of sequence b
+ * sees positions 0 .. seq_lens[b] - Nq + j.  q, out [B, Nq, H, 128] bf16 (strides in elements, multiples of 8), lse
+ * fp32 [B, Nq, H] contiguous or NULL (natural log; -inf, and an output row of zeros, where a row sees nothing).
+ * pages int32 [B, Hkv, list_width] with page_counts int32 [B, Hkv] (both contiguous): only the first
+ * page_counts[b][h] logical pages of the list are attended, in any order, one that occurs twice twice;
+ * NULL: all pages.  Scores, softmax state and sums are fp32.  Two launches (one where no sequence can be
+ * long enough to be split).  workspace: 256-byte aligned, at least aa_paged_attend_workspace_bytes() (which depends
+ * on the current device); it need not be zeroed, and calls that may overlap need workspaces of their own.
+ */
+typedef struct aa_paged_attend {
+    aa_paged_cache_t cache;
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t q_stride_b, q_stride_n, q_stride_h;
+    int64_t o_stride_b, o_stride_n, o_stride_h;
+    const int32_t *pages, *page_counts;
+    void *workspace;
+    size_t workspace_bytes;
+    double sm_scale;                   /* 0 => D^-0.5 */
+    int32_t list_width, Nq, H;
+    int32_t reserved;
+} aa_paged_attend_t;
+int aa_paged_attend_workspace_bytes(const aa_paged_attend_t *a, size_t *bytes);
+int aa_paged_attend(const aa_paged_attend_t *a, void *stream);
+
+/*
+ * The pages of every sequence and KV head to attend: the first keep_first and the last keep_last pages, then those of
+ * the best score, `top` in all (all of them where a sequence has no more).  A page's score is the maximum over
+ * the KV head's query rows of (query code . key code) * query scale, times the page's key_code_scale, where a
+ * query row q [B, Nq, H, 128] has the scale max|q| * (1 / 127) and the codes rint(q / scale); a tie goes to the lower page.
+ * out int32 [B, Hkv, top]: logical pages, ascending, -1 behind counts int32 [B, Hkv].  keep_last >= 1 covers a last
+ * page that is not full and so has no codes yet; keep_first + keep_last <= top.  Only the table, the lengths and
+ * the shape fields of `cache` are read, the pool pointers and strides are not.  One launch.
+ */
+typedef struct aa_page_select {
+    aa_paged_cache_t cache;
+    const void *q;
+    int64_t q_stride_b, q_stride_n, q_stride_h;
+    const int8_t *key_codes;
+    const float  *key_code_scales;
+    int32_t *out, *counts;
+    int32_t Nq, H, top, keep_first, keep_last;
+    int32_t reserved;
+} aa_page_select_t;
+int aa_page_select(const aa_page_select_t *a, void *stream);
 
 const char *aa_strerror(int code);
 /* Text of the last CUDA error this library saw on the calling thread. */
