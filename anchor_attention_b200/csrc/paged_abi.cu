@@ -83,17 +83,68 @@ aa::paged::Cache view(const aa_paged_cache_t& c, int log2_page) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
+// ---- tensor maps: a pool [pages, Hkv, page_size, 128] as a 4-D map, dimension 0 the row, the others by increasing
+// stride (a dimension of size 1 last, where its stride does not matter).  A copy takes 128 bytes of `box` rows.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return reinterpret_cast<EncodeTiledFn>(ok ? p : nullptr);
+    }();
+    return fn;
+}
+
+int make_page_map(CUtensorMap* map, const aa::paged::Pool& pool, const aa_paged_cache_t& c, int box, aa::paged::MapOrder* order) {
+    const EncodeTiledFn encode = encode_tiled();
+    if (!encode) return record_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled entry point");
+    struct Dim {
+        int64_t stride;                            // bytes
+        cuuint64_t size;
+        int* place;
+    };
+    Dim d[3] = {{pool.row, (cuuint64_t)c.page_size, &order->row}, {pool.head, (cuuint64_t)c.Hkv, &order->head},
+                {pool.page, (cuuint64_t)c.pages, &order->page}};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if ((d[j].size != 1 && d[j].stride < d[i].stride) || (d[i].size == 1 && d[j].size != 1)) {
+                const Dim x = d[i];
+                d[i] = d[j];
+                d[j] = x;
+            }
+    const bool fp8 = c.cache_dtype == AA_E4M3;
+    const cuuint64_t row_bytes = fp8 ? 128 : 256;
+    const cuuint64_t sizes[4] = {128, d[0].size, d[1].size, d[2].size};
+    cuuint64_t strides[3];
+    cuuint32_t boxes[4] = {fp8 ? 128u : 64u, 1, 1, 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 3; ++i) {
+        strides[i] = d[i].size == 1 ? (i ? strides[i - 1] * sizes[i] : row_bytes) : (cuuint64_t)d[i].stride;
+        *d[i].place = i;
+        if (d[i].place == &order->row) boxes[i + 1] = (cuuint32_t)box;
+    }
+    const CUresult r = encode(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool.ptr, sizes,
+                              strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? AA_OK : record_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled (strides of the page pools)");
+}
+
 // ---- attention: how a call is cut up
 struct AttendPlan {
     int log2_page, rows, row_tiles, tiles8;       // tiles8: tiles of 8 rows one CTA holds (1 .. 4)
-    int ctas;
+    int ctas, unit_keys;
     bool split;                                   // whether an entry can be cut at all
     size_t o_off, ml_off, cut_off, bytes;
 };
 
-template <bool FP8, int NT>
+template <bool FP8, int RW>
 cudaError_t allow_smem() {
-    return cudaFuncSetAttribute(aa::paged::paged_attend_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(aa::paged::paged_attend_kernel<FP8, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 aa::paged::kSmemBytes);
 }
 
@@ -121,7 +172,14 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
     pl.tiles8 = (int)ceil_div(ceil_div(pl.rows, pl.row_tiles), 8);
     const int64_t entries = (int64_t)c.B * c.Hkv * pl.row_tiles;
     const int64_t keys = (int64_t)(a->pages ? a->list_width : c.table_width) * c.page_size;
-    const int64_t units = ceil_div(keys, aa::paged::kUnitKeys);
+    const bool fp8 = c.cache_dtype == AA_E4M3;
+    static const int unit_keys[2][4] = {
+        {aa::paged::Shape<false, 1>::kUnitKeys, aa::paged::Shape<false, 2>::kUnitKeys, aa::paged::Shape<false, 3>::kUnitKeys,
+         aa::paged::Shape<false, 4>::kUnitKeys},
+        {aa::paged::Shape<true, 1>::kUnitKeys, aa::paged::Shape<true, 2>::kUnitKeys, aa::paged::Shape<true, 3>::kUnitKeys,
+         aa::paged::Shape<true, 4>::kUnitKeys}};
+    pl.unit_keys = unit_keys[fp8][pl.tiles8 - 1];
+    const int64_t units = ceil_div(keys, pl.unit_keys);
     if (entries * units > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
     const int64_t most = (int64_t)dev.sms * aa::paged::kCtasPerSm;
     pl.ctas = (int)(entries * units < most ? entries * units : most);
@@ -135,15 +193,17 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
     return AA_OK;
 }
 
-template <bool FP8, int NT>
-int launch_attend(const aa::paged::AttendParams& p, const AttendPlan& pl, cudaStream_t st) {
-    aa::paged::paged_attend_kernel<FP8, NT><<<pl.ctas, aa::paged::kThreads, aa::paged::kSmemBytes, st>>>(p);
+template <bool FP8, int RW>
+int launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const aa::paged::AttendParams& p, const AttendPlan& pl,
+                  cudaStream_t st) {
+    aa::paged::paged_attend_kernel<FP8, RW>
+        <<<pl.ctas, aa::paged::Shape<FP8, RW>::kThreads, aa::paged::kSmemBytes, st>>>(k_map, v_map, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_attend");
     if (!pl.split) return AA_OK;
     // the join kernel's launch overlaps the attention kernel's end; it waits on the device for its results
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pl.ctas - 1, 8 * NT < pl.rows ? 8 * NT : pl.rows);
+    cfg.gridDim = dim3(pl.ctas - 1, 8 * RW < pl.rows ? 8 * RW : pl.rows);
     cfg.blockDim = dim3(aa::paged::kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -151,18 +211,19 @@ int launch_attend(const aa::paged::AttendParams& p, const AttendPlan& pl, cudaSt
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, pl.ctas, 8 * NT);
+    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, pl.ctas, 8 * RW);
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_join");
     return AA_OK;
 }
 
 template <bool FP8>
-int launch_attend_rows(const aa::paged::AttendParams& p, const AttendPlan& pl, cudaStream_t st) {
+int launch_attend_rows(const CUtensorMap& km, const CUtensorMap& vm, const aa::paged::AttendParams& p, const AttendPlan& pl,
+                       cudaStream_t st) {
     switch (pl.tiles8) {
-        case 1: return launch_attend<FP8, 1>(p, pl, st);
-        case 2: return launch_attend<FP8, 2>(p, pl, st);
-        case 3: return launch_attend<FP8, 3>(p, pl, st);
-        default: return launch_attend<FP8, 4>(p, pl, st);
+        case 1: return launch_attend<FP8, 1>(km, vm, p, pl, st);
+        case 2: return launch_attend<FP8, 2>(km, vm, p, pl, st);
+        case 3: return launch_attend<FP8, 3>(km, vm, p, pl, st);
+        default: return launch_attend<FP8, 4>(km, vm, p, pl, st);
     }
 }
 
@@ -181,6 +242,7 @@ int aa_paged_check_status(uint32_t* status, void* stream) {
     if (!word) return AA_OK;
     e = cudaMemsetAsync(status, 0, sizeof(word), st);
     if (e != cudaSuccess) return record_cuda_error(e, "cudaMemsetAsync(status)");
+    if (word & aa::paged::kStatusTimeout) return AA_ERR_DEVICE_TIMEOUT;
     return word & aa::paged::kStatusBadPage ? AA_ERR_BAD_PAGE : AA_ERR_TOO_LONG;
 }
 
@@ -286,7 +348,14 @@ int aa_paged_attend(const aa_paged_attend_t* a, void* stream) {
     p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
     p.cut_entry = reinterpret_cast<int32_t*>(ws + pl.cut_off);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return c.cache_dtype == AA_E4M3 ? launch_attend_rows<true>(p, pl, st) : launch_attend_rows<false>(p, pl, st);
+    const int box = c.page_size < pl.unit_keys ? c.page_size : pl.unit_keys;
+    p.log2_box = 31 - __builtin_clz((unsigned)box);
+    CUtensorMap k_map, v_map;
+    rc = make_page_map(&k_map, p.c.k, c, box, &p.k_order);
+    if (!rc) rc = make_page_map(&v_map, p.c.v, c, box, &p.v_order);
+    if (rc) return rc;
+    return c.cache_dtype == AA_E4M3 ? launch_attend_rows<true>(k_map, v_map, p, pl, st)
+                                    : launch_attend_rows<false>(k_map, v_map, p, pl, st);
 }
 
 int aa_page_select(const aa_page_select_t* a, void* stream) {

@@ -6,19 +6,22 @@
 // 2 * rows * (bytes per value)^-1 multiply-adds -- 8 operations a byte for a group of four and bf16 -- so the
 // cache has to stream from HBM at full rate and everything else has to stay out of its way.
 //
-// Work split.  An entry is one (sequence, KV head, tile of rows); its keys are cut into units of 64.  All
+// Work split.  An entry is one (sequence, KV head, tile of up to 32 rows); its keys are cut into units.  All
 // units of all entries form one line that is cut into as many equal ranges as there are CTAs, whatever the
 // lengths: a batch of unequal sequences and a single long one fill the GPU alike.  Where a cut falls inside an
 // entry, the CTAs on its sides leave (maximum, sum, unnormalised row) and join_kernel adds them up
 // in the order of the keys; so results depend on the lengths alone, not on timing.
 //
-// Inside a CTA every warp streams its own 16 keys of a unit through its own ring in shared memory
-// (cp.async, no barrier between warps in the loop) and keeps its own softmax state; the four states are
-// added up where an entry ends.  Scores are computed transposed, S^T = K Q^T: the keys fill the 16 rows of the
-// matrix instruction and 8 queries its columns, so a group of 4 wastes half of a tile of 8 instead of three
-// quarters of one of 16; the probabilities then need one 8x8 transpose to become the operand of
-// O^T = V^T P^T.  mma.sync is enough: a tensor-core tile of 128 rows would be filled with padding, and the
-// instruction rate needed is a sixth of what mma.sync reaches.
+// Inside a CTA a producer warp walks the units: it looks up their pages and has the TMA copy them (128-byte swizzle)
+// into a ring of stages, one ahead of the other.  The keys of a unit go to KW lanes of RW warps, 16 keys a
+// lane; every lane keeps a softmax state of its own, and the states are added up where an entry ends.  The RW
+// warps of a lane own eight query rows each.  Everything but the arithmetic is the producer's: with the copies and
+// page lookups in the computing warps (cp.async, a ring for every lane) an e4m3 tile took 467 warp instructions and
+// the instruction rate was the limit, at 4.9 TB/s.
+// Scores are computed transposed, S^T = K Q^T: the keys fill the 16 rows of the matrix instruction and 8 queries its
+// columns, so a group of 4 wastes half of a tile of 8 instead of three quarters of one of 16; the
+// probabilities then need one 8x8 transpose to become the operand of O^T = V^T P^T.  mma.sync is enough: a
+// tensor-core tile of 128 rows would be filled with padding, and the tensor pipe is busy a seventh of the time.
 //
 // Accuracy.  Scores, softmax state and outputs are held in 32 bits.  With bf16 pages a probability goes into
 // the second product as the sum of two bf16 values (15 bits), so that only the output is rounded to 8;
@@ -26,22 +29,40 @@
 // code is exact and a probability keeps 11 bits; queries are scaled by a power of two per row to fit f16.
 #pragma once
 #include "paged_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace aa {
 namespace paged {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kTileKeys = 16;                       // keys of one warp and step
-constexpr int kUnitKeys = kWarps * kTileKeys;       // keys of one CTA and step
+constexpr int kTileKeys = 16;                       // keys of one lane and step
 constexpr int kCombStride = 132;                    // floats; 132 keeps the transposed writes off each other's banks
-constexpr int kCombBytes = kWarps * 8 * kCombStride * 4;
+constexpr int kCombRows = 32;                       // rows of partial results a round of adding up holds
+constexpr int kCombBytes = kCombRows * kCombStride * 4;
 constexpr int kRingBytes = 96 * 1024;               // with the join buffer, two CTAs fill an SM's shared memory
 constexpr int kCtasPerSm = 2;
+constexpr int kSegments = 16;                       // entries of a CTA's range whose lengths are kept at hand
+constexpr int kMiscBytes = 512;
+constexpr int kSmemBytes = kRingBytes + kCombBytes + kMiscBytes;
 
-constexpr int tile_bytes(bool fp8) { return kTileKeys * kD * (fp8 ? 1 : 2); }
-constexpr int stages(bool fp8) { return kRingBytes / (kWarps * 2 * tile_bytes(fp8)); }
-constexpr int kSmemBytes = kRingBytes + kCombBytes;
+// The warps of a CTA (and one more, the producer) and the stages of its ring.
+template <bool FP8, int RW>
+struct Shape {
+    static constexpr int kLanes = RW == 1 ? (FP8 ? 8 : 4) : RW == 2 ? 4 : 2;
+    static constexpr int kWarps = kLanes * RW;
+    static constexpr int kThreads = (kWarps + 1) * 32;
+    static constexpr int kUnitKeys = kLanes * kTileKeys;
+    static constexpr int kParts = FP8 ? 2 : 4;                       // of 128 bytes a key: keys, values, or halves of them
+    static constexpr int kPartBytes = kUnitKeys * 128;
+    static constexpr int kUnitBytes = kParts * kPartBytes;
+    static constexpr int kStages = kRingBytes / kUnitBytes < 8 ? kRingBytes / kUnitBytes : 8;
+    static constexpr int kRows = 8 * RW;
+    static constexpr int kRoundRows = kCombRows / kLanes < kRows ? kCombRows / kLanes : kRows;   // rows added up at a time
+};
+
+// How the coordinates of a copy are ordered in a pool's tensor map (dimension 0 is the row of 128 values).
+struct MapOrder {
+    int row, head, page;                            // 0 .. 2
+};
 
 struct AttendParams {
     Cache c;
@@ -54,16 +75,18 @@ struct AttendParams {
     const int32_t* page_counts;                     // [B, Hkv]
     int list_width;
     int B, H, Hkv, Hg, nq;
-    int rows, row_tiles;                            // rows = nq * Hg in tiles of 8 * NT
+    int rows, row_tiles;                            // rows = nq * Hg, in tiles of 8 * RW
     float scale_log2;                               // softmax scale times log2 e
-    float* part_o;                                  // [ctas, 2, 8 NT, 128]
-    float2* part_ml;                                // [ctas, 2, 8 NT]
+    float* part_o;                                  // [ctas, 2, 8 RW, 128]
+    float2* part_ml;                                // [ctas, 2, 8 RW]
     int32_t* cut_entry;                             // [ctas]: the entry a CTA's range starts inside of, or -1
+    MapOrder k_order, v_order;
+    int log2_box;                                   // keys of one copy: the smaller of page and unit
 };
 
 // Keys an entry streams over (list entries count as whole pages) and the units they make; an empty one still
 // makes a unit, so that some CTA writes its zeros.
-__device__ __forceinline__ int entry_units(const AttendParams& p, int e) {
+__device__ __forceinline__ int entry_units(const AttendParams& p, int e, int unit_keys) {
     const int bh = e / p.row_tiles;
     int64_t keys;
     if (p.pages) {
@@ -71,27 +94,32 @@ __device__ __forceinline__ int entry_units(const AttendParams& p, int e) {
     } else {
         keys = seq_len(p.c, bh / p.Hkv);
     }
-    return max(1, (int)((keys + kUnitKeys - 1) / kUnitKeys));
+    return max(1, (int)((keys + unit_keys - 1) / unit_keys));
 }
 
-// One warp's place in the line of units.
+// One lane's place in the line of units.
 struct Cursor {
     int entry, unit, units;                         // unit: next one of the entry
     int b, h, len;
 };
 
-__device__ __forceinline__ void enter(const AttendParams& p, Cursor& c, int entry) {
+__device__ __forceinline__ void enter(const AttendParams& p, Cursor& c, int entry, int unit_keys, const int2* segments, int first_entry) {
     c.entry = entry;
-    c.units = entry_units(p, entry);
     const int bh = entry / p.row_tiles;
     c.b = bh / p.Hkv;
     c.h = bh - c.b * p.Hkv;
-    c.len = seq_len(p.c, c.b);
+    if (entry - first_entry < kSegments) {
+        c.units = segments[entry - first_entry].x;
+        c.len = segments[entry - first_entry].y;
+    } else {
+        c.units = entry_units(p, entry, unit_keys);
+        c.len = seq_len(p.c, c.b);
+    }
 }
 
-// Where the 16 keys of (cursor, warp) are: the pool page, or -1 for none; `pos` their first position.
-__device__ __forceinline__ int locate(const AttendParams& p, const Cursor& c, int warp, int& pos) {
-    const int64_t flat = ((int64_t)c.unit * kWarps + warp) * kTileKeys;
+// Where the 16 keys of (cursor, lane) are: the pool page, or -1 for none; `pos` their first position.
+__device__ __forceinline__ int locate(const AttendParams& p, const Cursor& c, int lanes, int lane, int& pos) {
+    const int64_t flat = ((int64_t)c.unit * lanes + lane) * kTileKeys;
     int logical = (int)(flat >> p.c.log2_page);
     const int within = (int)(flat & ((1 << p.c.log2_page) - 1));
     if (p.pages) {
@@ -111,78 +139,57 @@ __device__ __forceinline__ int locate(const AttendParams& p, const Cursor& c, in
     return page;
 }
 
-template <bool FP8>
+// A 16-byte chunk of a lane's row (0 .. 15) in its part of a stage: the TMA's 128-byte swizzle, and for bf16 the second
+// half of a row's 256 bytes in the next part.
+template <bool FP8, int RW>
 __device__ __forceinline__ uint32_t tile_addr(uint32_t base, int row, int chunk) {
-    // 16-byte chunks of a row, XORed with the row so that eight rows of a column of chunks fall on different banks
-    return base + row * (FP8 ? kD : 2 * kD) + ((chunk ^ (row & 7)) << 4);
+    return base + (FP8 ? 0 : (chunk >> 3) * Shape<FP8, RW>::kPartBytes) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// One warp copies the keys and values of its 16 positions; rows behind the sequence's end become zeros.
-template <bool FP8>
-__device__ __forceinline__ void load_tile(const AttendParams& p, uint32_t slot, int page, int h, int pos, int len, int lane) {
-    constexpr int kChunks = FP8 ? 8 : 16;
-    const int row0 = pos & ((1 << p.c.log2_page) - 1);
-    const uint8_t* k = p.c.k.ptr + page * p.c.k.page + h * p.c.k.head + row0 * p.c.k.row;
-    const uint8_t* v = p.c.v.ptr + page * p.c.v.page + h * p.c.v.head + row0 * p.c.v.row;
-    const int live = min(kTileKeys, len - pos);
-#pragma unroll
-    for (int i = 0; i < kTileKeys * kChunks / 32; ++i) {
-        const int row = i * (32 / kChunks) + lane / kChunks, chunk = lane % kChunks;
-        const bool in = row < live;
-        cp_async16(tile_addr<FP8>(slot, row, chunk), k + (in ? row * p.c.k.row : 0) + chunk * 16, in ? 16 : 0);
-        cp_async16(tile_addr<FP8>(slot + tile_bytes(FP8), row, chunk), v + (in ? row * p.c.v.row : 0) + chunk * 16,
-                   in ? 16 : 0);
-    }
-}
-
-// Query rows of an entry as operands of S^T = K Q^T, f16 and scaled by a power of two for e4m3 pages.
-// Lane (g, t) holds row g of each tile of 8: the values that meet a lane's K values in step s.
-template <bool FP8, int NT>
+// Eight query rows of an entry as operands of S^T = K Q^T.  Lane (g, t) holds row g: the values that meet its K values
+// in step s.
 struct Queries {
-    uint32_t f[NT][8][2];
-    float unscale[NT][2];                           // of this lane's score columns 2t, 2t + 1 (e4m3 only)
+    uint32_t f[8][2];
+    float unscale[2];                               // of this lane's score columns 2t, 2t + 1 (e4m3 only)
 };
 
-template <bool FP8, int NT>
-__device__ __forceinline__ void load_queries(const AttendParams& p, int b, int h, int row0, int lane, Queries<FP8, NT>& qf) {
+template <bool FP8>
+__device__ __forceinline__ void fetch_queries(const AttendParams& p, const Cursor& c, int row0, int lane, Queries& qf) {
     const int g = lane >> 2, t = lane & 3;
+    const int r = row0 + g;
+    const bool in = r < p.rows;
+    const int j = in ? r / p.Hg : 0, i = in ? r - j * p.Hg : 0;
+    const uint32_t* src =
+        reinterpret_cast<const uint32_t*>(p.q + c.b * p.q_sb + j * p.q_sn + (int64_t)(c.h * p.Hg + i) * p.q_sh);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = row0 + n * 8 + g;
-        const bool in = r < p.rows;
-        const int j = in ? r / p.Hg : 0, i = in ? r - j * p.Hg : 0;
-        const uint32_t* src =
-            reinterpret_cast<const uint32_t*>(p.q + b * p.q_sb + j * p.q_sn + (int64_t)(h * p.Hg + i) * p.q_sh);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const int at = FP8 ? s * 8 + t * 2 : s * 8 + t;          // in pairs of values
-            qf.f[n][s][0] = in ? src[at] : 0u;
-            qf.f[n][s][1] = in ? src[at + (FP8 ? 1 : 4)] : 0u;
-        }
-        if (FP8) {
-            uint32_t big = 0;                       // largest |q| of the row, as bf16 bits
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    big = max(big, max(qf.f[n][s][w] & 0x7FFFu, (qf.f[n][s][w] >> 16) & 0x7FFFu));
-            big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-            big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-            // the row times 2^-e has its largest value in [256, 512): f16 then keeps 2^-32 of it
-            const int expo = max(min((int)(big >> 7), 254) - 127 - 8, -126);
-            const float down = __uint_as_float((uint32_t)(127 - expo) << 23);
-            const float up = __uint_as_float((uint32_t)(127 + expo) << 23);
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t x = qf.f[n][s][w];
-                    qf.f[n][s][w] = pack_f16x2(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xFFFF0000u) * down);
-                }
-            qf.unscale[n][0] = __shfl_sync(0xFFFFFFFFu, up, t * 8);
-            qf.unscale[n][1] = __shfl_sync(0xFFFFFFFFu, up, t * 8 + 4);
-        }
+    for (int s = 0; s < 8; ++s) {
+        const int at = FP8 ? s * 8 + t * 2 : s * 8 + t;              // in pairs of values
+        qf.f[s][0] = in ? src[at] : 0u;
+        qf.f[s][1] = in ? src[at + (FP8 ? 1 : 4)] : 0u;
     }
+}
+
+// bf16 -> f16, scaled by a power of two so that a row's largest value lies in [256, 512): f16 then keeps 2^-32 of it.
+__device__ __forceinline__ void queries_to_f16(int lane, Queries& qf) {
+    uint32_t big = 0;                               // largest |q| of the row, as bf16 bits
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) big = max(big, max(qf.f[s][w] & 0x7FFFu, (qf.f[s][w] >> 16) & 0x7FFFu));
+    big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+    big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+    const int expo = max(min((int)(big >> 7), 254) - 127 - 8, -126);
+    const float down = __uint_as_float((uint32_t)(127 - expo) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + expo) << 23);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t x = qf.f[s][w];
+            qf.f[s][w] = pack_f16x2(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xFFFF0000u) * down);
+        }
+    qf.unscale[0] = __shfl_sync(0xFFFFFFFFu, up, (lane & 3) * 8);
+    qf.unscale[1] = __shfl_sync(0xFFFFFFFFu, up, (lane & 3) * 8 + 4);
 }
 
 // Accumulates P^T into the accumulators of one group of values: a = 16 values x 16 keys.  MASK: only the columns
@@ -213,28 +220,27 @@ __device__ __forceinline__ void value_mma(float (&o)[4], const uint32_t (&a)[4],
 
 // O^T += V^T P^T for one tile.  MASK: the values of this lane's keys (2t, 2t+1) and (2t+8, 2t+9) are masked by
 // keep0, keep1, and only the columns in `own` are added to.
-template <bool FP8, int NT, bool MASK>
-__device__ __forceinline__ void value_product(uint32_t v_slot, int lane, const uint32_t (&ph)[NT][2], const uint32_t (&pl)[NT][2],
-                                              float (&o)[NT][8][4], uint32_t keep0, uint32_t keep1, const bool (&own)[NT][2]) {
+template <bool FP8, int RW, bool MASK>
+__device__ __forceinline__ void value_product(uint32_t v_slot, int lane, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
+                                              float (&o)[8][4], uint32_t keep0, uint32_t keep1, const bool (&own)[2]) {
     const int mi = lane >> 3;
     if (!FP8) {
         const int key = (lane & 7) + ((mi >> 1) << 3);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint32_t a[4];
-            ldmatrix4_trans(tile_addr<false>(v_slot, key, 2 * i + (mi & 1)), a);
+            ldmatrix4_trans(tile_addr<false, RW>(v_slot, key, 2 * i + (mi & 1)), a);
             if (MASK) {
                 a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1;
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) value_mma<FP8, MASK>(o[n][i], a, ph[n], pl[n], own[n]);
+            value_mma<FP8, MASK>(o[i], a, ph, pl, own);
         }
     } else {
         const int key = (lane & 7) + ((mi & 1) << 3);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             uint32_t x[4];
-            ldmatrix4_trans(tile_addr<true>(v_slot, key, i + (mi >> 1)), x);
+            ldmatrix4_trans(tile_addr<true, RW>(v_slot, key, i + (mi >> 1)), x);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 // a pair of 16-bit units = (value 2g, 2g+1) of keys 2t and 2t+1: regroup by value
@@ -243,11 +249,22 @@ __device__ __forceinline__ void value_product(uint32_t v_slot, int lane, const u
                 if (MASK) {
                     a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1;
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) value_mma<FP8, MASK>(o[n][i + u], a, ph[n], pl[n], own[n]);
+                value_mma<FP8, MASK>(o[i + u], a, ph, pl, own);
             }
         }
     }
+}
+
+// A finished row, four values a thread; a row that has seen nothing is 0.
+__device__ __forceinline__ void store_row(__nv_bfloat16* to, int lane, const float4& acc, float sum, float v_scale) {
+    const float f = sum == 0.0f ? 0.0f : v_scale / sum;
+    const bool none = sum == 0.0f;
+    reinterpret_cast<uint2*>(to)[lane] = make_uint2(pack_bf16x2(none ? 0.0f : acc.x * f, none ? 0.0f : acc.y * f),
+                                                    pack_bf16x2(none ? 0.0f : acc.z * f, none ? 0.0f : acc.w * f));
+}
+// The natural logarithm of a softmax sum from its maximum (log2 units) and the sum behind it.
+__device__ __forceinline__ float log_sum(float top, float sum) {
+    return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // The value index (0 .. 127) of accumulator o[.][i][2 * up] in lane row g.
@@ -256,42 +273,55 @@ __device__ __forceinline__ int value_index(int i, int up, int g) {
     return FP8 ? 16 * i + 2 * g + up : 16 * i + 8 * up + g;
 }
 
-template <bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attend_kernel(const __grid_constant__ AttendParams p) {
-    constexpr int kStages = stages(FP8);
-    constexpr int kRows = 8 * NT;
-    extern __shared__ __align__(128) uint8_t paged_smem[];
-    uint8_t* smem = paged_smem;
-    __shared__ int s_warp_sum[kWarps];
-    __shared__ int s_entry, s_unit;
-    __shared__ int s_pos[kWarps][kStages];          // first position of the tile in a ring slot, -1: none
+template <bool FP8, int RW>
+__global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
+    paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                        const __grid_constant__ AttendParams p) {
+    using S = Shape<FP8, RW>;
+    constexpr int kStages = S::kStages;
+    extern __shared__ __align__(1024) uint8_t paged_attend_smem[];
+    float* comb = reinterpret_cast<float*>(paged_attend_smem + kRingBytes);
+    // the last 512 bytes: barriers, lengths of this range's entries, tile positions of the stages, scratch of the start
+    const uint32_t ring = smem_u32(paged_attend_smem);
+    const uint32_t bars = ring + kRingBytes + kCombBytes;
+    auto full = [&](uint32_t stage) { return bars + 8u * stage; };
+    auto empty = [&](uint32_t stage) { return bars + 8u * (kStages + stage); };
+    int2* segments = reinterpret_cast<int2*>(paged_attend_smem + kRingBytes + kCombBytes + 16 * kStages);
+    int* s_pos = reinterpret_cast<int*>(segments + kSegments);                    // [stages][lanes], -1: no keys
+    int* s_sum = s_pos + S::kLanes * kStages;                                     // [warps], then (entry, unit)
+    volatile int* abort_flag = s_sum + S::kWarps + 3;
+    static_assert(16 * kStages + kSegments * 8 + (S::kLanes * kStages + S::kWarps + 4) * 4 <= kMiscBytes, "the last 512 bytes");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * (kRingBytes / kWarps);
-    float* comb = reinterpret_cast<float*>(smem + kRingBytes);
 
-#if __CUDA_ARCH__ >= 900
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-#endif
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::mbar_init(full(i), 1);
+            tc::mbar_init(empty(i), S::kWarps);
+        }
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+    }
 
     // ---- this CTA's range of the line of units
     const int entries = p.B * p.Hkv * p.row_tiles;
-    const int chunk = (entries + kThreads - 1) / kThreads;
+    const int chunk = (entries + S::kThreads - 1) / S::kThreads;
+    const int my_first = tid * chunk, my_end = min(entries, my_first + chunk);
     int mine = 0;
-    for (int e = tid * chunk; e < min(entries, (tid + 1) * chunk); ++e) mine += entry_units(p, e);
+    for (int e = my_first; e < my_end; ++e) mine += entry_units(p, e, S::kUnitKeys);
     int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const int x = __shfl_up_sync(0xFFFFFFFFu, incl, d);
         if (lane >= d) incl += x;
     }
-    if (lane == 31) s_warp_sum[warp] = incl;
+    if (lane == 31) s_sum[warp] = incl;
     __syncthreads();
     int before = incl - mine, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_warp_sum[w];
-        total += s_warp_sum[w];
+    for (int w = 0; w < S::kWarps + 1; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
     }
     const int ctas = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= ctas) {
@@ -299,246 +329,294 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attend_kernel(cons
         return;
     }
     const int begin = (int)((int64_t)total * blockIdx.x / ctas);
-    int left = (int)((int64_t)total * (blockIdx.x + 1) / ctas) - begin;     // units to do, at least one
+    const int end = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
     if (begin >= before && begin < before + mine) {
-        int e = tid * chunk, at = before;
-        for (int n = entry_units(p, e); at + n <= begin; n = entry_units(p, e)) {
+        int e = my_first, at = before;
+        for (int n = entry_units(p, e, S::kUnitKeys); at + n <= begin; n = entry_units(p, e, S::kUnitKeys)) {
             at += n;
             ++e;
         }
-        s_entry = e;
-        s_unit = begin - at;
+        s_sum[S::kWarps + 1] = e;
+        s_sum[S::kWarps + 2] = begin - at;
     }
     __syncthreads();
-
-    Cursor ahead;                                   // the next tile to copy
-    enter(p, ahead, s_entry);
-    ahead.unit = s_unit;
-    Cursor now = ahead;                             // the tile to compute
-    if (tid == 0) p.cut_entry[blockIdx.x] = s_unit > 0 ? s_entry : -1;
+    const int first_entry = s_sum[S::kWarps + 1], first_unit = s_sum[S::kWarps + 2];
+    if (before < end && before + mine > begin) {
+        int at = before;
+        for (int e = my_first; e < my_end && at < end && e - first_entry < kSegments; ++e) {
+            const int n = chunk == 1 ? mine : entry_units(p, e, S::kUnitKeys);
+            if (e >= first_entry) segments[e - first_entry] = make_int2(n, seq_len(p.c, e / p.row_tiles / p.Hkv));
+            at += n;
+        }
+    }
+    if (tid == 0) p.cut_entry[blockIdx.x] = first_unit > 0 ? first_entry : -1;
     if (blockIdx.x == 0)                            // the row of the block table bounds a sequence: report a longer one
-        for (int b = tid; b < p.B; b += kThreads)
+        for (int b = tid; b < p.B; b += S::kThreads)
             if (p.c.seq_lens[b] > ((int64_t)p.c.table_width << p.c.log2_page)) raise_status(p.c, kStatusTooLong);
-    int to_copy = left;
-    int pos_ahead = 0, page_ahead = locate(p, ahead, warp, pos_ahead);
-    uint32_t slot_in = 0, slot_out = 0;             // ring slots, modulo kStages
+    __syncthreads();
 
-    auto copy_next = [&]() {
-        if (to_copy > 0) {
-            if (lane == 0) s_pos[warp][slot_in] = page_ahead >= 0 ? pos_ahead : -1;
-            if (page_ahead >= 0)
-                load_tile<FP8>(p, ring + slot_in * (2 * tile_bytes(FP8)), page_ahead, ahead.h, pos_ahead, ahead.len, lane);
-            if (--to_copy > 0) {
-                if (++ahead.unit == ahead.units) {
-                    enter(p, ahead, ahead.entry + 1);
-                    ahead.unit = 0;
+    int left = end - begin;                         // units to do, at least one
+    Cursor now;
+    enter(p, now, first_entry, S::kUnitKeys, segments, first_entry);
+    now.unit = first_unit;
+
+    if (warp == S::kWarps) {
+        // ================================================== producer
+        // lane i < kLanes looks up tile i of the unit; lane 8 * part + box issues a copy
+        const int boxes = S::kUnitKeys >> p.log2_box, box_bytes = 128 << p.log2_box;
+        const int box = lane & 7, part = lane >> 3;
+        const bool issues = part < S::kParts && box < boxes;
+        const bool of_values = part >= S::kParts / 2;
+        const CUtensorMap* map = of_values ? &v_map : &k_map;
+        const MapOrder order = of_values ? p.v_order : p.k_order;
+        const int x = FP8 ? 0 : (part & 1) * 64;
+        const uint32_t box_at = part * S::kPartBytes + box * box_bytes;
+        int pos = 0, page = lane < S::kLanes ? locate(p, now, S::kLanes, lane, pos) : -1;
+        uint32_t stage = 0, parity = 1;             // of the stage's previous use: the first pass waits for nothing
+        for (int i = 0; i < left; ++i) {
+            tc::mbar_wait(empty(stage), parity, abort_flag);
+            __syncwarp();
+            if (*abort_flag) break;
+            const int first_tile = (box << p.log2_box) / kTileKeys;
+            const int box_page = __shfl_sync(0xFFFFFFFFu, page, first_tile & 31);
+            const int box_pos = __shfl_sync(0xFFFFFFFFu, pos, first_tile & 31);
+            const bool issue = issues && box_page >= 0;
+            const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, issue)) * box_bytes;
+            if (lane < S::kLanes) s_pos[stage * S::kLanes + lane] = page >= 0 ? pos : -1;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_expect_tx(full(stage), bytes);
+            __syncwarp();
+            if (issue) {
+                const int row = box_pos & ((1 << p.c.log2_page) - 1);
+                int at[3];
+#pragma unroll
+                for (int d = 0; d < 3; ++d) at[d] = order.row == d ? row : order.head == d ? now.h : box_page;
+                tc::tma_load_4d(ring + stage * S::kUnitBytes + box_at, map, full(stage), x, at[0], at[1], at[2]);
+            }
+            if (i + 1 < left) {
+                if (++now.unit == now.units) {
+                    enter(p, now, now.entry + 1, S::kUnitKeys, segments, first_entry);
+                    now.unit = 0;
                 }
-                page_ahead = locate(p, ahead, warp, pos_ahead);   // used at the next step: its latency is hidden
+                page = lane < S::kLanes ? locate(p, now, S::kLanes, lane, pos) : -1;   // used after the next wait
+            }
+            if (++stage == kStages) {
+                stage = 0;
+                parity ^= 1;
             }
         }
-        slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
-        cp_async_commit();
-    };
-    for (int s = 0; s < kStages - 1; ++s) copy_next();
+        if (*abort_flag) {
+            // a wait gave up: let the copies in flight land before shared memory is handed on
+            for (int i = 0; i < kStages; ++i) tc::mbar_wait(full(i), 0, abort_flag), tc::mbar_wait(full(i), 1, abort_flag);
+            if (lane == 0) raise_status(p.c, kStatusTimeout);
+        }
+        return;
+    }
+
+    // ====================================================== the computing warps
+    const int g = lane >> 2, t = lane & 3;
+    const int kl = warp / RW, rw = warp % RW;       // key lane; which eight rows
+    auto compute_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(S::kWarps * 32) : "memory"); };
+    uint32_t stage = 0, parity = 0;
+    Queries qf;
+    fetch_queries<FP8>(p, now, now.entry % p.row_tiles * S::kRows + rw * 8, lane, qf);
 
     while (left > 0) {
         // ---- one entry, or the part of it that lies in this range
-        const int row0 = (now.entry % p.row_tiles) * kRows;
+        const int row_base = now.entry % p.row_tiles * S::kRows;
+        const int row0 = row_base + rw * 8;         // this warp's rows
         const int unit0 = now.unit;
         const int todo = min(left, now.units - now.unit);
-        Queries<FP8, NT> qf;
-        load_queries<FP8, NT>(p, now.b, now.h, row0, lane, qf);
+        if (FP8) queries_to_f16(lane, qf);
         const float c0 = p.scale_log2 * (FP8 ? p.c.k_scale[now.h] : 1.0f);
-        float o[NT][8][4], m[NT][2], l[NT][2];
-        int limit[NT][2];                           // this lane's two rows of a tile see positions below it
+        const float scale[2] = {FP8 ? c0 * qf.unscale[0] : c0, FP8 ? c0 * qf.unscale[1] : c0};
+        float o[8][4], m[2], l[2];
+        int limit[2];                               // this lane's two rows see positions below it
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][i][x] = 0.0f;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                m[n][x] = -INFINITY;
-                l[n][x] = 0.0f;
-                limit[n][x] = now.len - p.nq + 1 + min(row0 + n * 8 + 2 * t + x, p.rows - 1) / p.Hg;
-            }
-        }
+            for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
         const int all_see = now.len - p.nq + 1;     // every row sees the positions below it
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+            limit[x] = all_see + min(row0 + 2 * t + x, p.rows - 1) / p.Hg;
+        }
 
-        for (int step = 0; step < todo; ++step, ++now.unit) {
-            cp_async_wait<kStages - 2>();
-            __syncwarp();
-            const int pos = s_pos[warp][slot_out];
-            copy_next();                            // into the slot that the step before has read
-            if (pos >= 0) {
-                const uint32_t slot = ring + slot_out * (2 * tile_bytes(FP8));
-                float s[NT][4];
+        for (int step = 0; step < todo; ++step) {
+            const uint32_t free_bar = empty(stage);
+            const bool landed = tc::mbar_wait(full(stage), parity, abort_flag);
+            const int pos = landed ? s_pos[stage * S::kLanes + kl] : -1;
+            const uint32_t slot = ring + stage * S::kUnitBytes + kl * (kTileKeys * 128);
+            if (++stage == kStages) {
+                stage = 0;
+                parity ^= 1;
+            }
+            if (__any_sync(0xFFFFFFFFu, pos < 0)) {
+                if (lane == 0) tc::mbar_arrive(free_bar);
+                continue;
+            }
+            // ---- scores, in two sums: s = keys (g, g, g+8, g+8) x rows (2t, 2t+1, 2t, 2t+1)
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (!FP8) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) s[n][x] = 0.0f;
-                if (!FP8) {
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        uint32_t a[4];
-                        ldmatrix4(tile_addr<false>(slot, lane & 15, 2 * ks + (lane >> 4)), a);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_bf16(s[n], a, qf.f[n][ks][0], qf.f[n][ks][1]);
-                    }
-                } else {
-#pragma unroll
-                    for (int ks = 0; ks < 8; ks += 2) {
-                        uint32_t x[4];
-                        ldmatrix4(tile_addr<true>(slot, lane & 15, ks + (lane >> 4)), x);
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            uint32_t a[4] = {e4m3x2_to_f16x2(x[2 * u]), e4m3x2_to_f16x2(x[2 * u + 1]),
-                                             e4m3x2_to_f16x2(x[2 * u] >> 16), e4m3x2_to_f16x2(x[2 * u + 1] >> 16)};
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_f16(s[n], a, qf.f[n][ks + u][0], qf.f[n][ks + u][1]);
-                        }
-                    }
+                for (int ks = 0; ks < 8; ks += 2) {
+                    uint32_t a[4], a2[4];
+                    ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + (lane >> 4)), a);
+                    ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + 2 + (lane >> 4)), a2);
+                    mma_bf16(s, a, qf.f[ks][0], qf.f[ks][1]);
+                    mma_bf16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
                 }
-                // ---- softmax step: s[n] = keys (g, g, g+8, g+8) x rows (2t, 2t+1, 2t, 2t+1)
-                const bool edge = pos + kTileKeys > all_see;
-                uint32_t ph[NT][2], pl[NT][2];
+            } else {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float scale = FP8 ? c0 * qf.unscale[n][x & 1] : c0;
-                        s[n][x] *= scale;
-                        if (edge && pos + g + (x >> 1) * 8 >= limit[n][x & 1]) s[n][x] = -INFINITY;
-                    }
-                    float corr[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float top = fmaxf(s[n][x], s[n][x + 2]);
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                        const float m_new = fmaxf(m[n][x], top);
-                        const float ref = m_new == -INFINITY ? 0.0f : m_new;   // a row that has seen nothing yet
-                        corr[x] = fast_exp2(m[n][x] - ref);
-                        m[n][x] = m_new;
-                        s[n][x] = fast_exp2(s[n][x] - ref);
-                        s[n][x + 2] = fast_exp2(s[n][x + 2] - ref);
-                        l[n][x] = l[n][x] * corr[x] + (s[n][x] + s[n][x + 2]);
-                    }
-                    if (corr[0] != 1.0f || corr[1] != 1.0f) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) o[n][i][x] *= corr[x & 1];
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float a = s[n][2 * half], b = s[n][2 * half + 1];
-                        if (FP8) {
-                            ph[n][half] = movmatrix_trans(pack_f16x2(a, b));
-                            pl[n][half] = 0;
-                        } else {
-                            // the upper 8 bits, and the rest -- a hair more of it, so that a probability above
-                            // zero has two parts above zero and an infinite value stays infinite, not NaN
-                            const uint32_t hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-                            const float more = 1.0f + 0x1p-23f;
-                            ph[n][half] = movmatrix_trans(hi);
-                            pl[n][half] = movmatrix_trans(pack_bf16x2(fmaf(a, more, -__uint_as_float(hi << 16)),
-                                                                      fmaf(b, more, -__uint_as_float(hi & 0xFFFF0000u))));
-                        }
-                    }
-                }
-                const uint32_t v_slot = slot + tile_bytes(FP8);
-                bool own[NT][2] = {};
-                if (!edge || p.nq == 1) {
-                    value_product<FP8, NT, false>(v_slot, lane, ph, pl, o, 0, 0, own);
-                } else {
-                    // Keys that only some of the rows may see: a masked probability of zero does not protect a
-                    // row from an infinity or NaN in a value, so every new token gets a product of its own with
-                    // the values behind its position cleared (one or two tiles of an entry).
-                    const int j1 = (min(row0 + kRows, p.rows) - 1) / p.Hg;
-#pragma unroll 1
-                    for (int j = row0 / p.Hg; j <= j1; ++j) {
-                        const int seen = all_see + j - pos;                     // keys of the tile this token sees
-                        if (seen <= 0) continue;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) own[n][x] = (row0 + n * 8 + 2 * t + x) / p.Hg == j;
-                        const uint32_t k0 = (2 * t < seen ? 0xFFFFu : 0u) | (2 * t + 1 < seen ? 0xFFFF0000u : 0u);
-                        const uint32_t k1 = (2 * t + 8 < seen ? 0xFFFFu : 0u) | (2 * t + 9 < seen ? 0xFFFF0000u : 0u);
-                        value_product<FP8, NT, true>(v_slot, lane, ph, pl, o, k0, k1, own);
-                    }
+                for (int ks = 0; ks < 8; ks += 2) {
+                    uint32_t x[4];
+                    ldmatrix4(tile_addr<true, RW>(slot, lane & 15, ks + (lane >> 4)), x);
+                    const uint32_t a[4] = {e4m3x2_to_f16x2(x[0]), e4m3x2_to_f16x2(x[1]), e4m3x2_to_f16x2(x[0] >> 16),
+                                           e4m3x2_to_f16x2(x[1] >> 16)};
+                    const uint32_t a2[4] = {e4m3x2_to_f16x2(x[2]), e4m3x2_to_f16x2(x[3]), e4m3x2_to_f16x2(x[2] >> 16),
+                                            e4m3x2_to_f16x2(x[3] >> 16)};
+                    mma_f16(s, a, qf.f[ks][0], qf.f[ks][1]);
+                    mma_f16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
                 }
             }
-            __syncwarp();                           // the slot has been read
-            slot_out = slot_out + 1 == kStages ? 0 : slot_out + 1;
-        }
-        left -= todo;
-
-        // ---- add up the warps' states, eight rows at a time
-        const bool whole = unit0 == 0 && now.unit == now.units;
-        const int64_t part = ((int64_t)blockIdx.x * 2 + (unit0 > 0 ? 0 : 1)) * kRows;
-        const float v_scale = FP8 ? p.c.v_scale[now.h] : 1.0f;
+            // ---- softmax step
+            const bool edge = pos + kTileKeys > all_see;
+            float corr[2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (row0 + n * 8 >= p.rows) break;
-            float* mine_o = comb + warp * 8 * kCombStride;
+            for (int x = 0; x < 4; ++x) {
+                s[x] = (s[x] + s2[x]) * scale[x & 1];
+                if (edge && pos + g + (x >> 1) * 8 >= limit[x & 1]) s[x] = -INFINITY;
+            }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                float sum = l[n][x];
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-                if (g == 0) {
-                    mine_o[(2 * t + x) * kCombStride + kD] = m[n][x];
-                    mine_o[(2 * t + x) * kCombStride + kD + 1] = sum;
-                }
+                float top = fmaxf(s[x], s[x + 2]);
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                const float m_new = fmaxf(m[x], top);
+                const float ref = m_new == -INFINITY ? 0.0f : m_new;       // a row that has seen nothing yet
+                corr[x] = fast_exp2(m[x] - ref);
+                m[x] = m_new;
+                s[x] = fast_exp2(s[x] - ref);
+                s[x + 2] = fast_exp2(s[x + 2] - ref);
+                l[x] = l[x] * corr[x] + (s[x] + s[x + 2]);
+            }
+            if (__any_sync(0xFFFFFFFFu, corr[0] != 1.0f || corr[1] != 1.0f)) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int up = 0; up < 2; ++up)
-                        mine_o[(2 * t + x) * kCombStride + value_index<FP8>(i, up, g)] = o[n][i][2 * up + x];
+                    for (int x = 0; x < 4; ++x) o[i][x] *= corr[x & 1];
             }
-            __syncthreads();
+            uint32_t ph[2], pl[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float a = s[2 * half], b = s[2 * half + 1];
+                if (FP8) {
+                    ph[half] = movmatrix_trans(pack_f16x2(a, b));
+                    pl[half] = 0;
+                } else {
+                    // the upper 8 bits, and the rest -- a hair more of it, so that a probability above
+                    // zero has two parts above zero and an infinite value stays infinite, not NaN
+                    const uint32_t hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+                    const float more = 1.0f + 0x1p-23f;
+                    ph[half] = movmatrix_trans(hi);
+                    pl[half] = movmatrix_trans(pack_bf16x2(fmaf(a, more, -__uint_as_float(hi << 16)),
+                                                           fmaf(b, more, -__uint_as_float(hi & 0xFFFF0000u))));
+                }
+            }
+            const uint32_t v_slot = slot + S::kUnitBytes / 2;
+            bool own[2] = {false, false};
+            if (!edge) {
+                value_product<FP8, RW, false>(v_slot, lane, ph, pl, o, 0, 0, own);
+            } else {
+                // Keys behind the end, or that only some of the rows may see: a masked probability of zero does not
+                // protect a row from an infinity or NaN in a value, so every new token gets a product of its own
+                // with the values behind its position cleared (one or two tiles of an entry).
+                const int j1 = (min(row0 + 8, p.rows) - 1) / p.Hg;
 #pragma unroll 1
-            for (int rr = 0; rr < 8; ++rr) {
-                const int r = row0 + n * 8 + rr;
+                for (int j = row0 / p.Hg; j <= j1; ++j) {
+                    const int seen = all_see + j - pos;                         // keys of the tile this token sees
+                    if (seen <= 0) continue;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) own[x] = (row0 + 2 * t + x) / p.Hg == j;
+                    const uint32_t k0 = (2 * t < seen ? 0xFFFFu : 0u) | (2 * t + 1 < seen ? 0xFFFF0000u : 0u);
+                    const uint32_t k1 = (2 * t + 8 < seen ? 0xFFFFu : 0u) | (2 * t + 9 < seen ? 0xFFFF0000u : 0u);
+                    value_product<FP8, RW, true>(v_slot, lane, ph, pl, o, k0, k1, own);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(free_bar);
+        }
+        left -= todo;
+        now.unit += todo;
+
+        // ---- add up the lanes' states, kRoundRows rows at a time; a warp takes a row, a thread four values
+        const bool whole = unit0 == 0 && now.unit == now.units;
+        const int64_t part = ((int64_t)blockIdx.x * 2 + (unit0 > 0 ? 0 : 1)) * S::kRows;
+        const float v_scale = FP8 ? p.c.v_scale[now.h] : 1.0f;
+        const int b_done = now.b, h_done = now.h;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            l[x] += __shfl_xor_sync(0xFFFFFFFFu, l[x], 4);
+            l[x] += __shfl_xor_sync(0xFFFFFFFFu, l[x], 8);
+            l[x] += __shfl_xor_sync(0xFFFFFFFFu, l[x], 16);
+        }
+        if (left > 0) {                             // the next entry's queries arrive meanwhile
+            enter(p, now, now.entry + 1, S::kUnitKeys, segments, first_entry);
+            now.unit = 0;
+            fetch_queries<FP8>(p, now, now.entry % p.row_tiles * S::kRows + rw * 8, lane, qf);
+        }
+        for (int base = 0; base < S::kRows && row_base + base < p.rows; base += S::kRoundRows) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int at = rw * 8 + 2 * t + x - base;
+                if (at >= 0 && at < S::kRoundRows) {
+                    float* to = comb + (kl * S::kRoundRows + at) * kCombStride;
+                    if (g == 0) {
+                        to[kD] = m[x];
+                        to[kD + 1] = l[x];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int up = 0; up < 2; ++up) to[value_index<FP8>(i, up, g)] = o[i][2 * up + x];
+                }
+            }
+            compute_sync();
+            for (int rr = warp; rr < min(S::kRoundRows, S::kRows - base); rr += S::kWarps) {
+                const int r = row_base + base + rr;
                 if (r >= p.rows) break;
-                float top = -INFINITY;
+                float top = -INFINITY, weight[S::kLanes];
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, comb[(w * 8 + rr) * kCombStride + kD]);
+                for (int w = 0; w < S::kLanes; ++w) {
+                    weight[w] = comb[(w * S::kRoundRows + rr) * kCombStride + kD];
+                    top = fmaxf(top, weight[w]);
+                }
                 const float ref = top == -INFINITY ? 0.0f : top;
-                float sum = 0.0f, acc = 0.0f;
+                float sum = 0.0f;
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float* from = comb + (w * 8 + rr) * kCombStride;
-                    const float f = fast_exp2(from[kD] - ref);
+                for (int w = 0; w < S::kLanes; ++w) {
+                    const float* from = comb + (w * S::kRoundRows + rr) * kCombStride;
+                    const float f = fast_exp2(weight[w] - ref);
+                    const float4 x = reinterpret_cast<const float4*>(from)[lane];
                     sum += f * from[kD + 1];
-                    acc += f * from[tid];
+                    acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
                 }
                 if (whole) {
-                    const int j = r / p.Hg, head = now.h * p.Hg + (r - j * p.Hg);
-                    p.out[now.b * p.o_sb + j * p.o_sn + head * p.o_sh + tid] =
-                        __float2bfloat16_rn(sum == 0.0f ? 0.0f : acc * v_scale / sum);
-                    if (p.lse && tid == 0)
-                        p.lse[((int64_t)now.b * p.nq + j) * p.H + head] =
-                            sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                    const int j = r / p.Hg, head = h_done * p.Hg + (r - j * p.Hg);
+                    store_row(p.out + b_done * p.o_sb + j * p.o_sn + head * p.o_sh, lane, acc, sum, v_scale);
+                    if (p.lse && lane == 0) p.lse[((int64_t)b_done * p.nq + j) * p.H + head] = log_sum(top, sum);
                 } else {
-                    p.part_o[(part + n * 8 + rr) * kD + tid] = acc;
-                    if (tid == 0) p.part_ml[part + n * 8 + rr] = make_float2(top, sum);
+                    reinterpret_cast<float4*>(p.part_o + (part + base + rr) * kD)[lane] = acc;
+                    if (lane == 0) p.part_ml[part + base + rr] = make_float2(top, sum);
                 }
             }
-            __syncthreads();
-        }
-        if (left > 0) {
-            enter(p, now, now.entry + 1);
-            now.unit = 0;
+            compute_sync();
         }
     }
-    cp_async_wait<0>();
 }
 
 // Adds up the parts of the entries that a cut of the line went through.  Block (c, r): if CTA c's range starts
@@ -553,9 +631,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     __shared__ float4 s_acc[kJoinThreads / 32][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c = blockIdx.x + 1, rr = blockIdx.y;
-#if __CUDA_ARCH__ >= 900
     asm volatile("griddepcontrol.wait;" ::: "memory");
-#endif
     const int entry = p.cut_entry[c];
     if (entry < 0 || p.cut_entry[c - 1] == entry) return;
     const int row0 = (entry % p.row_tiles) * tile_rows;
@@ -599,17 +675,17 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     }
     s_acc[warp][lane] = acc;
     __syncthreads();
-    if (tid < kD) {
-        float v = 0.0f;
+    if (warp == 0) {
+        acc = s_acc[0][lane];
 #pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; ++w) v += reinterpret_cast<const float*>(&s_acc[w][0])[tid];
+        for (int w = 1; w < kJoinThreads / 32; ++w) {
+            const float4 x = s_acc[w][lane];
+            acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+        }
         const int bh = entry / p.row_tiles, b = bh / p.Hkv, h = bh - b * p.Hkv;
         const int j = r / p.Hg, head = h * p.Hg + (r - j * p.Hg);
-        const float v_scale = FP8 ? p.c.v_scale[h] : 1.0f;
-        p.out[b * p.o_sb + j * p.o_sn + head * p.o_sh + tid] =
-            __float2bfloat16_rn(sum == 0.0f ? 0.0f : v * v_scale / sum);
-        if (p.lse && tid == 0)
-            p.lse[((int64_t)b * p.nq + j) * p.H + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        store_row(p.out + b * p.o_sb + j * p.o_sn + head * p.o_sh, lane, acc, sum, FP8 ? p.c.v_scale[h] : 1.0f);
+        if (p.lse && lane == 0) p.lse[((int64_t)b * p.nq + j) * p.H + head] = log_sum(top, sum);
     }
 }
 

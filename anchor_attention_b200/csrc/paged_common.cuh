@@ -15,6 +15,7 @@ namespace paged {
 constexpr int kMaxNew = 16;              // new tokens a sequence brings to one attention call, at most
 constexpr uint32_t kStatusBadPage = 1;   // a page number outside the pool, or a list entry outside the sequence
 constexpr uint32_t kStatusTooLong = 2;   // a sequence longer than its row of the block table, or than the rotary tables
+constexpr uint32_t kStatusTimeout = 4;   // a bounded wait gave up
 
 // An 8-bit code's scale is the largest magnitude times this: the product, not a division, is the definition.
 constexpr float kInv127 = 1.0f / 127.0f;
