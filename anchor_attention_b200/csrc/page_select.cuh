@@ -7,19 +7,24 @@
 // cut.  The first and the last pages of a sequence are always kept; the rest go by score, ties to the lower
 // page, and come out in ascending order.
 //
-// One block per (sequence, KV head): warps score 16 pages at a time with the 8-bit matrix instruction (pages as
-// its 16 rows, 8 query rows as its columns), the scores stay in shared memory as ordered 32-bit keys, four
-// counting passes over 8 bits each find the last key that gets in, and one more pass writes the list.
+// A cluster of blocks works on one (sequence, KV head).  Its warps score 16 pages at a time with the 8-bit matrix
+// instruction (pages as its 16 rows, 8 query rows as its columns) and leave the scores as ordered 32-bit keys in the
+// first block's shared memory; that block finds the last key that gets in by counting over 11 + 11 + 10 bits and writes the
+// list.  The scores are a few dependent loads per page, so a small batch is a matter of latency: eight blocks
+// share a sequence there, and each warp has 32 pages' loads in flight.
 #pragma once
 #include "paged_common.cuh"
 
 namespace aa {
 namespace paged {
 
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxSelectRows = 256;                 // new tokens * group: 33 KB of query codes
 constexpr int kMaxSelectPages = 40960;              // 160 KB of keys
+constexpr int kMaxSelectCluster = 8;
+constexpr int kBins = 2048;                         // of one counting pass
+constexpr int kBinsPerThread = kBins / kSelectThreads;
 
 struct SelectParams {
     Cache c;                                        // table, seq_lens, pages, log2_page, status
@@ -33,8 +38,12 @@ struct SelectParams {
 };
 
 __host__ __device__ inline int select_row_tiles(int rows) { return (rows + 7) / 8; }
+// keys (rounded up to whole vectors for every thread), counts, query codes and scales
+__host__ __device__ inline int select_key_slots(int table_width) {
+    return (table_width + 4 * kSelectThreads - 1) / (4 * kSelectThreads) * (4 * kSelectThreads);
+}
 inline size_t select_smem_bytes(int rows, int table_width) {
-    return (size_t)select_row_tiles(rows) * 8 * (kD + 4) + (size_t)table_width * 4;
+    return (size_t)select_key_slots(table_width) * 4 + kBins * 4 + (size_t)select_row_tiles(rows) * 8 * (kD + 4);
 }
 
 // larger score, larger key; +0 and -0 alike
@@ -43,31 +52,122 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const __grid_constant__ SelectParams p) {
-    extern __shared__ __align__(128) uint8_t paged_smem[];
-    uint8_t* smem = paged_smem;
-    __shared__ int s_hist[256];
-    __shared__ int s_warp[2][kSelectWarps];
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// the address in block 0 of the cluster of a shared-memory address of this block
+__device__ __forceinline__ uint32_t in_first_block(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+}
+
+// Sum of x over the threads below this one; `total`: over all.  Two barriers.
+__device__ __forceinline__ int2 block_scan(int2 x, int2& total, int2* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int2 incl = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, incl.x, d), b = __shfl_up_sync(0xFFFFFFFFu, incl.y, d);
+        if (lane >= d) {
+            incl.x += a;
+            incl.y += b;
+        }
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int2 before = make_int2(incl.x - x.x, incl.y - x.y);
+    total = make_int2(0, 0);
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) {
+        const int2 n = s_warp[w];
+        if (w < warp) {
+            before.x += n.x;
+            before.y += n.y;
+        }
+        total.x += n.x;
+        total.y += n.y;
+    }
+    __syncthreads();
+    return before;
+}
+
+// A page's mean key as a matrix operand: lane (g, t) holds the bytes 16 t .. 16 t + 15 and 64 + 16 t .. 64 + 16 t + 15 of
+// pages g and g + 8 of its 16.
+struct PageTile {
+    uint4 lo[2], hi[2];
+    float scale[2];
+    int page[2];
+};
+
+__global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const __grid_constant__ SelectParams p, int cluster) {
+    extern __shared__ __align__(128) uint8_t page_select_smem[];
+    __shared__ int2 s_warp[kSelectWarps];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int bh = blockIdx.x, b = bh / p.Hkv, h = bh - b * p.Hkv;
+    const int bh = blockIdx.x / cluster, b = bh / p.Hkv, h = bh - b * p.Hkv;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     const int padded = select_row_tiles(p.rows) * 8;
-    uint32_t* s_q = reinterpret_cast<uint32_t*>(smem);                            // [padded][32] four codes each
-    float* s_scale = reinterpret_cast<float*>(smem + (size_t)padded * kD);        // [padded]
-    uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + (size_t)padded * (kD + 4));
+    uint32_t* s_key = reinterpret_cast<uint32_t*>(page_select_smem);
+    int* s_hist = reinterpret_cast<int*>(s_key + select_key_slots(p.c.table_width));
+    uint32_t* s_q = reinterpret_cast<uint32_t*>(s_hist + kBins);                  // [padded][32] four codes each
+    float* s_scale = reinterpret_cast<float*>(s_q + padded * 32);                 // [padded]
 
     const int len = seq_len(p.c, b);
-    if (tid == 0 && h == 0 && p.c.seq_lens[b] > ((int64_t)p.c.table_width << p.c.log2_page)) raise_status(p.c, kStatusTooLong);
+    if (tid == 0 && h == 0 && rank == 0 && p.c.seq_lens[b] > ((int64_t)p.c.table_width << p.c.log2_page))
+        raise_status(p.c, kStatusTooLong);
     const int live = (int)(((int64_t)len + (1 << p.c.log2_page) - 1) >> p.c.log2_page);
     const int count = min(live, p.top);
     int32_t* out = p.out + (int64_t)bh * p.top;
-    if (tid == 0) p.counts[bh] = count;
-    for (int i = count + tid; i < p.top; i += kSelectThreads) out[i] = -1;
-    if (live <= p.top) {
-        for (int i = tid; i < live; i += kSelectThreads) out[i] = i;
+    if (rank == 0) {
+        if (tid == 0) p.counts[bh] = count;
+        for (int i = count + tid; i < p.top; i += kSelectThreads) out[i] = -1;
+    }
+    if (live <= p.top) {                            // the same for all blocks of the cluster
+        if (rank == 0)
+            for (int i = tid; i < live; i += kSelectThreads) out[i] = i;
         return;
     }
+    if (cluster > 1) cluster_arrive();              // every block has started: before the first store to another
+
+    // ---- page numbers of this warp's first two tiles, while the queries arrive
+    const int stride = cluster * kSelectWarps * 16;
+    auto find = [&](int base, PageTile& x) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int logical = base + g + 8 * i;
+            x.page[i] = logical < live ? p.c.table[b * p.c.table_stride + logical] : -1;
+        }
+    };
+    auto load = [&](int base, PageTile& x) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if ((uint32_t)x.page[i] >= (uint32_t)p.c.pages) {
+                if (base + g + 8 * i < live) raise_status(p.c, kStatusBadPage);
+                x.page[i] = -1;
+            }
+            x.lo[i] = x.hi[i] = make_uint4(0, 0, 0, 0);
+            x.scale[i] = 0.0f;
+            if (x.page[i] >= 0) {
+                const int64_t at = (int64_t)x.page[i] * p.Hkv + h;
+                x.lo[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + t);
+                x.hi[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + 4 + t);
+                x.scale[i] = __ldg(p.code_scales + at);
+            }
+        }
+    };
+    const int base0 = (rank * kSelectWarps + warp) * 16;
+    PageTile x0, x1;
+    find(base0, x0);
+    find(base0 + stride, x1);
 
     // ---- query rows in 8 bits
     for (int r = warp; r < padded; r += kSelectWarps) {
@@ -92,128 +192,127 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const __gri
         s_q[r * 32 + lane] = packed;
         if (lane == 0) s_scale[r] = r < p.rows ? scale : 0.0f;
     }
+    load(base0, x0);
+    load(base0 + stride, x1);
     __syncthreads();
+    if (cluster > 1) cluster_wait();
 
-    // ---- score 16 pages a warp; a lane's words of a page: bytes 16 t .. 16 t + 15 and 64 + 16 t .. 64 + 16 t + 15
+    // ---- scores
     const int row_tiles = padded / 8;
-    for (int base = warp * 16; base < live; base += kSelectWarps * 16) {
-        uint32_t a[2][8];
-        float scale[2];
-        int page[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int logical = base + g + 8 * x;
-            page[x] = -1;
-            if (logical < live) {
-                page[x] = pool_page(p.c, b, logical);
-                if (page[x] < 0) raise_status(p.c, kStatusBadPage);
-            }
-            uint4 u = make_uint4(0, 0, 0, 0), w = u;
-            scale[x] = 0.0f;
-            if (page[x] >= 0) {
-                const int64_t at = (int64_t)page[x] * p.Hkv + h;
-                u = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + t);
-                w = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + 4 + t);
-                scale[x] = __ldg(p.code_scales + at);
-            }
-            a[x][0] = u.x; a[x][1] = u.y; a[x][2] = u.z; a[x][3] = u.w;
-            a[x][4] = w.x; a[x][5] = w.y; a[x][6] = w.z; a[x][7] = w.w;
-        }
+    const uint32_t keys_at = cluster > 1 ? in_first_block(smem_u32(s_key)) : 0;
+    auto score = [&](int base, const PageTile& x) {
         float best[2] = {-INFINITY, -INFINITY};
+        const uint32_t a0[4] = {x.lo[0].x, x.lo[1].x, x.lo[0].y, x.lo[1].y};
+        const uint32_t a1[4] = {x.lo[0].z, x.lo[1].z, x.lo[0].w, x.lo[1].w};
+        const uint32_t a2[4] = {x.hi[0].x, x.hi[1].x, x.hi[0].y, x.hi[1].y};
+        const uint32_t a3[4] = {x.hi[0].z, x.hi[1].z, x.hi[0].w, x.hi[1].w};
         for (int n = 0; n < row_tiles; ++n) {
             const uint4* q = reinterpret_cast<const uint4*>(s_q + (n * 8 + g) * 32);
             const uint4 u = q[t], w = q[4 + t];
             int d[4] = {0, 0, 0, 0};
-            const uint32_t a0[4] = {a[0][0], a[1][0], a[0][1], a[1][1]};
-            const uint32_t a1[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
-            const uint32_t a2[4] = {a[0][4], a[1][4], a[0][5], a[1][5]};
-            const uint32_t a3[4] = {a[0][6], a[1][6], a[0][7], a[1][7]};
             mma_s8(d, a0, u.x, u.y);
             mma_s8(d, a1, u.z, u.w);
             mma_s8(d, a2, w.x, w.y);
             mma_s8(d, a3, w.z, w.w);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int r = n * 8 + 2 * t + (x & 1);
-                if (r < p.rows) best[x >> 1] = fmaxf(best[x >> 1], __fmul_rn((float)d[x], s_scale[r]));
+            for (int i = 0; i < 4; ++i) {
+                const int r = n * 8 + 2 * t + (i & 1);
+                if (r < p.rows) best[i >> 1] = fmaxf(best[i >> 1], __fmul_rn((float)d[i], s_scale[r]));
             }
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            best[x] = fmaxf(best[x], __shfl_xor_sync(0xFFFFFFFFu, best[x], 1));
-            best[x] = fmaxf(best[x], __shfl_xor_sync(0xFFFFFFFFu, best[x], 2));
-            const int logical = base + g + 8 * x;
+        for (int i = 0; i < 2; ++i) {
+            best[i] = fmaxf(best[i], __shfl_xor_sync(0xFFFFFFFFu, best[i], 1));
+            best[i] = fmaxf(best[i], __shfl_xor_sync(0xFFFFFFFFu, best[i], 2));
+            const int logical = base + g + 8 * i;
             if (t == 0 && logical < live) {
-                uint32_t key = page[x] >= 0 ? order_key(__fmul_rn(best[x], scale[x])) : 0u;
+                uint32_t key = x.page[i] >= 0 ? order_key(__fmul_rn(best[i], x.scale[i])) : 0u;
                 if (logical < p.keep_first || logical >= live - p.keep_last) key = 0xFFFFFFFFu;
-                s_key[logical] = key;
+                if (cluster > 1)
+                    store_cluster(keys_at + logical * 4, key);
+                else
+                    s_key[logical] = key;
             }
+        }
+    };
+    for (int base = base0; base < live; base += 2 * stride) {
+        score(base, x0);
+        if (base + stride < live) score(base + stride, x1);
+        if (base + 2 * stride < live) {
+            find(base + 2 * stride, x0);
+            find(base + 3 * stride, x1);
+            load(base + 2 * stride, x0);
+            load(base + 3 * stride, x1);
         }
     }
+    if (cluster > 1) {
+        cluster_arrive();
+        cluster_wait();
+        if (rank > 0) return;
+    } else {
+        __syncthreads();
+    }
 
-    // ---- the count-th largest key, 8 bits at a time from the top
+    // ---- the count-th largest key, 11, 11 and 10 bits at a time from the top
     uint32_t prefix = 0;
     int need = count;                               // how many of the keys with this prefix get in
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+        const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+#pragma unroll
+        for (int i = 0; i < kBinsPerThread; ++i) s_hist[tid + i * kSelectThreads] = 0;
         __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
         for (int i = tid; i < live; i += kSelectThreads) {
             const uint32_t k = s_key[i];
-            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & digits], 1);
         }
         __syncthreads();
-        if (warp == 0) {                            // lane: bins 8 (31 - lane) .. + 7, the highest bins first
-            int sum = 0;
+        // thread: bins kBinsPerThread (threads - 1 - tid) .. + kBinsPerThread - 1, the highest bins first
+        const int bin0 = kBinsPerThread * (kSelectThreads - 1 - tid);
+        int bins[kBinsPerThread], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += s_hist[8 * (31 - lane) + i];
-            int incl = sum;
+        for (int i = 0; i < kBinsPerThread; ++i) sum += bins[i] = s_hist[bin0 + i];
+        int2 total;
+        int above = block_scan(make_int2(sum, 0), total, s_warp).x;               // keys in higher bins
+        if (above < need && above + sum >= need) {
+            int bin = kBinsPerThread - 1;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int x = __shfl_up_sync(0xFFFFFFFFu, incl, d);
-                if (lane >= d) incl += x;
-            }
-            int above = incl - sum;                 // keys in higher bins
-            if (above < need && incl >= need) {
-                int bin = 8 * (31 - lane) + 7;
-                while (above + s_hist[bin] < need) above += s_hist[bin--];
-                s_prefix = prefix | ((uint32_t)bin << shift);
-                s_need = need - above;
-            }
+            for (int i = kBinsPerThread - 1; i > 0; --i)
+                if (bin == i && above + bins[i] < need) {
+                    above += bins[i];
+                    bin = i - 1;
+                }
+            s_prefix = prefix | ((uint32_t)(bin0 + bin) << shift);
+            s_need = need - above;
         }
         __syncthreads();
         prefix = s_prefix;
         need = s_need;
     }
 
-    // ---- keys above the cut, and the first `need` of those equal to it, in the order of the pages
-    int done = 0, equal_done = 0;
-    for (int i0 = 0; i0 < live; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        const uint32_t k = i < live ? s_key[i] : 0u;
-        const bool more = i < live && k > prefix, equal = i < live && k == prefix;
-        const uint32_t m_more = __ballot_sync(0xFFFFFFFFu, more), m_equal = __ballot_sync(0xFFFFFFFFu, equal);
-        if (lane == 0) {
-            s_warp[0][warp] = __popc(m_more);
-            s_warp[1][warp] = __popc(m_equal);
-        }
-        __syncthreads();
-        int more_before = done, equal_before = equal_done;
+    // ---- keys above the cut, and the first `need` of those equal to it: a thread takes a run of keys
+    const int run = (live + 4 * kSelectThreads - 1) / (4 * kSelectThreads) * 4;
+    const int begin = min(tid * run, live), end = min(begin + run, live);
+    int2 mine = make_int2(0, 0), total;
+    for (int i = begin; i < end; i += 4) {
+        const uint4 k4 = *reinterpret_cast<const uint4*>(s_key + i);
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-        for (int w = 0; w < kSelectWarps; ++w) {
-            if (w < warp) {
-                more_before += s_warp[0][w];
-                equal_before += s_warp[1][w];
-            }
-            done += s_warp[0][w];
-            equal_done += s_warp[1][w];
+        for (int x = 0; x < 4; ++x) {
+            mine.x += i + x < end && k[x] > prefix;
+            mine.y += i + x < end && k[x] == prefix;
         }
-        const uint32_t below = (1u << lane) - 1u;
-        more_before += __popc(m_more & below);
-        equal_before += __popc(m_equal & below);
-        if (more || (equal && equal_before < need)) out[more_before + min(equal_before, need)] = i;
-        __syncthreads();
     }
+    int2 before = block_scan(mine, total, s_warp);
+    if (mine.x + mine.y > 0)
+        for (int i = begin; i < end; ++i) {
+            const uint32_t k = s_key[i];
+            if (k > prefix || (k == prefix && before.y < need)) out[before.x + min(before.y, need)] = i;
+            before.x += k > prefix;
+            before.y += k == prefix;
+        }
 }
 
 }  // namespace paged

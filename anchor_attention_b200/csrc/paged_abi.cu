@@ -189,7 +189,7 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
     pl.o_off = 0;
     pl.ml_off = align256(parts * aa::kD * sizeof(float));
     pl.cut_off = align256(pl.ml_off + parts * sizeof(float2));
-    pl.bytes = align256(pl.cut_off + pl.ctas * sizeof(int32_t));
+    pl.bytes = align256(pl.cut_off + pl.ctas * sizeof(int2));
     return AA_OK;
 }
 
@@ -211,7 +211,7 @@ int launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const aa::
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, pl.ctas, 8 * RW);
+    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, 8 * RW);
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_join");
     return AA_OK;
 }
@@ -346,7 +346,7 @@ int aa_paged_attend(const aa_paged_attend_t* a, void* stream) {
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
     p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
-    p.cut_entry = reinterpret_cast<int32_t*>(ws + pl.cut_off);
+    p.cuts = reinterpret_cast<int2*>(ws + pl.cut_off);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int box = c.page_size < pl.unit_keys ? c.page_size : pl.unit_keys;
     p.log2_box = 31 - __builtin_clz((unsigned)box);
@@ -393,8 +393,23 @@ int aa_page_select(const aa_page_select_t* a, void* stream) {
     p.keep_first = a->keep_first;
     p.keep_last = a->keep_last;
     const size_t smem = aa::paged::select_smem_bytes(p.rows, c.table_width);
-    aa::paged::page_select_kernel<<<c.B * c.Hkv, aa::paged::kSelectThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-    cudaError_t e = cudaGetLastError();
+    // Blocks for a sequence and head: more as long as they leave SMs idle and have pages for their warps.
+    int cluster = 1;
+    while (cluster < aa::paged::kMaxSelectCluster && (int64_t)c.B * c.Hkv * cluster < dev.sms &&
+           c.table_width > cluster * aa::paged::kSelectWarps * 16)
+        cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(c.B * c.Hkv * cluster));
+    cfg.blockDim = dim3(aa::paged::kSelectThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, aa::paged::page_select_kernel, p, cluster);
     return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch page_select");
 }
 

@@ -10,7 +10,7 @@
 // units of all entries form one line that is cut into as many equal ranges as there are CTAs, whatever the
 // lengths: a batch of unequal sequences and a single long one fill the GPU alike.  Where a cut falls inside an
 // entry, the CTAs on its sides leave (maximum, sum, unnormalised row) and join_kernel adds them up
-// in the order of the keys; so results depend on the lengths alone, not on timing.
+// in the order of the keys; results depend on the lengths alone, not on timing.
 //
 // Inside a CTA a producer warp walks the units: it looks up their pages and has the TMA copy them (128-byte swizzle)
 // into a ring of stages, one ahead of the other.  The keys of a unit go to KW lanes of RW warps, 16 keys a
@@ -79,7 +79,9 @@ struct AttendParams {
     float scale_log2;                               // softmax scale times log2 e
     float* part_o;                                  // [ctas, 2, 8 RW, 128]
     float2* part_ml;                                // [ctas, 2, 8 RW]
-    int32_t* cut_entry;                             // [ctas]: the entry a CTA's range starts inside of, or -1
+    int2* cuts;                                     // [ctas]: (entry, parts) where a CTA's range is the first to start
+                                                    // inside that entry, which the CTA before it began and `parts` CTAs
+                                                    // share; else (-1, 0)
     MapOrder k_order, v_order;
     int log2_box;                                   // keys of one copy: the smaller of page and unit
 };
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     }
     const int ctas = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= ctas) {
-        if (tid == 0) p.cut_entry[blockIdx.x] = -1;
+        if (tid == 0) p.cuts[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     const int begin = (int)((int64_t)total * blockIdx.x / ctas);
@@ -349,7 +351,6 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
             at += n;
         }
     }
-    if (tid == 0) p.cut_entry[blockIdx.x] = first_unit > 0 ? first_entry : -1;
     if (blockIdx.x == 0)                            // the row of the block table bounds a sequence: report a longer one
         for (int b = tid; b < p.B; b += S::kThreads)
             if (p.c.seq_lens[b] > ((int64_t)p.c.table_width << p.c.log2_page)) raise_status(p.c, kStatusTooLong);
@@ -359,6 +360,13 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     Cursor now;
     enter(p, now, first_entry, S::kUnitKeys, segments, first_entry);
     now.unit = first_unit;
+    if (tid == 0) {
+        // CTA c owns the units [total c / ctas, total (c + 1) / ctas), so unit u belongs to CTA ((u + 1) ctas - 1) / total
+        const int starts = begin - first_unit;
+        const bool leads = first_unit > 0 && (int)((int64_t)total * (blockIdx.x - 1) / ctas) <= starts;
+        const int last = (int)(((int64_t)(starts + now.units) * ctas - 1) / total);
+        p.cuts[blockIdx.x] = leads ? make_int2(first_entry, last - (int)blockIdx.x + 2) : make_int2(-1, 0);
+    }
 
     if (warp == S::kWarps) {
         // ================================================== producer
@@ -619,26 +627,24 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     }
 }
 
-// Adds up the parts of the entries that a cut of the line went through.  Block (c, r): if CTA c's range starts
-// inside an entry and no earlier one's starts inside the same, row r of that entry is c - 1's part (which began
-// it) and those of c, c + 1, ... as long as they start inside it.
+// Adds up the parts of the entries that a cut of the line went through.  Block (c - 1, r) takes row r of the entry that CTA
+// c leads (see `cuts`): CTA c - 1 began it, c, c + 1, ... start inside it.
 constexpr int kJoinThreads = 256;
 
 template <bool FP8>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ AttendParams p, int ctas, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ AttendParams p, int tile_rows) {
     __shared__ float s_weight[512];
     __shared__ float s_red[kJoinThreads / 32];
     __shared__ float4 s_acc[kJoinThreads / 32][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c = blockIdx.x + 1, rr = blockIdx.y;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int entry = p.cut_entry[c];
-    if (entry < 0 || p.cut_entry[c - 1] == entry) return;
+    const int2 cut = p.cuts[c];
+    const int entry = cut.x, parts = cut.y;         // parts i = 0 .. parts - 1 come from CTAs c - 1 + i
+    if (entry < 0) return;
     const int row0 = (entry % p.row_tiles) * tile_rows;
     const int r = row0 + rr;
     if (r >= p.rows) return;
-    int parts = 2;                                  // parts i = 0 .. parts - 1 come from CTAs c - 1 + i
-    while (c + parts - 1 < ctas && p.cut_entry[c + parts - 1] == entry) ++parts;
     auto index = [&](int i) { return ((int64_t)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * tile_rows + rr; };
 
     float top = -INFINITY;
