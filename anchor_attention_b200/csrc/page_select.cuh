@@ -107,7 +107,7 @@ struct PageTile {
     int page[2];
 };
 
-__global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const __grid_constant__ SelectParams p, int cluster) {
+__global__ void __launch_bounds__(kSelectThreads, 4) page_select_kernel(const __grid_constant__ SelectParams p, int cluster) {
     extern __shared__ __align__(128) uint8_t page_select_smem[];
     __shared__ int2 s_warp[kSelectWarps];
     __shared__ uint32_t s_prefix;

@@ -265,7 +265,6 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     for (const void* p : {a->key, a->value, a->query, (const void*)a->query_out, (const void*)a->key_out, (const void*)a->cos,
                           (const void*)a->sin})
         if (misaligned(p)) return AA_ERR_STRIDE;
-    if (2 * (int64_t)c.Hkv > 65535) return AA_ERR_TOO_LARGE;
 
     aa::paged::AppendParams p;
     p.c = view(c, log2_page);
@@ -287,7 +286,6 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     p.B = c.B;
     p.H = a->H;
     p.Hkv = c.Hkv;
-    p.Hg = a->query ? a->H / c.Hkv : 0;
     p.per_seq = a->cu_seqlens ? 0 : a->T / c.B;
     // n tokens touch at most (n - 1) / page_size + 2 pages, one token one page
     int64_t tasks;
@@ -296,12 +294,27 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     else
         tasks = p.per_seq == 1 ? c.B : c.B * ((p.per_seq - 1) / c.page_size + (int64_t)2);
     if (tasks > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
-    const dim3 grid((unsigned)tasks, (unsigned)(a->query ? 2 * c.Hkv : c.Hkv));
+    // one token a sequence: a block for every KV head, one for all queries; more tokens: see paged_append.cuh
+    const bool single = !a->cu_seqlens && p.per_seq == 1;
+    p.kv_heads = single ? 1 : 2;
+    p.q_heads = single ? (a->H < 64 ? a->H : 64) : 8;
+    p.kv_blocks = (int)ceil_div(c.Hkv, p.kv_heads);
+    p.staged = !single && c.page_size <= aa::paged::kStagedPage;
+    const int64_t q_blocks = a->query ? ceil_div(a->H, p.q_heads) : 0;
+    if (p.kv_blocks + q_blocks > 65535) return AA_ERR_TOO_LARGE;
+    const dim3 grid((unsigned)tasks, (unsigned)(p.kv_blocks + q_blocks));
+    const bool fp8 = c.cache_dtype == AA_E4M3;
+    const size_t smem = p.staged && p.codes ? (size_t)p.kv_heads * c.page_size * (fp8 ? 128 : 256) : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (c.cache_dtype == AA_E4M3)
-        aa::paged::paged_append_kernel<true><<<grid, aa::paged::kAppendThreads, 0, st>>>(p);
+    constexpr int kMany = aa::paged::kAppendThreads, kOne = aa::paged::kSingleThreads;
+    if (single && fp8)
+        aa::paged::paged_append_kernel<true, kOne><<<grid, kOne, 0, st>>>(p);
+    else if (single)
+        aa::paged::paged_append_kernel<false, kOne><<<grid, kOne, 0, st>>>(p);
+    else if (fp8)
+        aa::paged::paged_append_kernel<true, kMany><<<grid, kMany, smem, st>>>(p);
     else
-        aa::paged::paged_append_kernel<false><<<grid, aa::paged::kAppendThreads, 0, st>>>(p);
+        aa::paged::paged_append_kernel<false, kMany><<<grid, kMany, smem, st>>>(p);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch paged_append");
 }
@@ -395,7 +408,7 @@ int aa_page_select(const aa_page_select_t* a, void* stream) {
     const size_t smem = aa::paged::select_smem_bytes(p.rows, c.table_width);
     // Blocks for a sequence and head: more as long as they leave SMs idle and have pages for their warps.
     int cluster = 1;
-    while (cluster < aa::paged::kMaxSelectCluster && (int64_t)c.B * c.Hkv * cluster < dev.sms &&
+    while (cluster < aa::paged::kMaxSelectCluster && (int64_t)c.B * c.Hkv * cluster < 2 * dev.sms &&
            c.table_width > cluster * aa::paged::kSelectWarps * 16)
         cluster *= 2;
     cudaLaunchConfig_t cfg = {};

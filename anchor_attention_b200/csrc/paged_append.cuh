@@ -11,7 +11,9 @@
 // loses nothing, so codes do not depend on the order of the sum.
 //
 // The kernel moves bytes: 8 threads take a row of 256 bytes in 16-byte pieces, a thread owning the values d and
-// d + 64 of a rotation.
+// d + 64 of a rotation.  For prompts a block takes several heads of a page, so that a row's cosines and sines are read once
+// for all of them and two heads' loads are in flight while the page number arrives; a single token's append is
+// latency alone and takes a block for every head.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -20,8 +22,9 @@
 namespace aa {
 namespace paged {
 
-constexpr int kAppendThreads = 256;
-constexpr int kRowsAtOnce = kAppendThreads / 8;
+constexpr int kAppendThreads = 256;                // for prompts; a single token a sequence takes kSingleThreads
+constexpr int kSingleThreads = 128;
+constexpr int kStagedPage = 64;                     // pages up to this size are added up in shared memory
 
 struct Rows {                                       // [tokens, heads, 128] bf16, strides in elements
     __nv_bfloat16* ptr;
@@ -37,8 +40,10 @@ struct AppendParams {
     int rope_rows;
     int8_t* codes;                                  // [pages, Hkv, 128] or null
     float* code_scales;                             // [pages, Hkv]
-    int T, B, H, Hkv, Hg;
+    int T, B, H, Hkv;
+    int kv_heads, kv_blocks, q_heads;               // heads of a block; blocks y < kv_blocks take keys and values
     int per_seq;                                    // cu == null: tokens of every sequence
+    bool staged;                                    // shared memory holds a block's pages
 };
 
 // New positions [start, end) of a sequence (negative ones are padding and are left out) and its first token.
@@ -81,17 +86,34 @@ __device__ __forceinline__ void unpack8(const uint4& x, float (&f)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
-__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
+// Division by one number for many: q = x r with r = 1 / s rounded, then one step q + (x - q s) r.  The step gives the
+// correctly rounded quotient (P. Markstein, Computation of elementary functions on the IBM RISC System/6000
+// processor, 1990) as long as nothing overflows or vanishes; what is not in a safe range divides.
+struct Divisor {
+    float s, r;
+    bool plain;                                     // s in a range where r and the step's products are normal numbers
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+    return Divisor{s, __fdiv_rn(1.0f, s), s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7FFFFFu) != 0x7FFFFFu};
+}
+__device__ __forceinline__ float divide(float x, const Divisor& d) {
+    // below 2^-60 / 2^60 the quotient's code is 0 whatever its last bit, above (or not finite) it saturates or is NaN
+    if (!d.plain || !(fabsf(x) <= 0x1p60f)) return __fdiv_rn(x, d.s);
+    const float q = __fmul_rn(x, d.r);
+    return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
+}
+__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], const Divisor& d) {
     uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        w[i >> 2] |= (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(f[i], scale), __NV_SATFINITE, __NV_E4M3) << (8 * (i & 3));
+    for (int i = 0; i < 8; i += 2)
+        w[i >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(divide(f[i], d), divide(f[i + 1], d)), __NV_SATFINITE, __NV_E4M3)
+                     << (8 * (i & 3));
     return make_uint2(w[0], w[1]);
 }
 __device__ __forceinline__ void load_piece(const Rows& r, int token, int head, int c, uint4& lo, uint4& hi) {
     const uint4* src = reinterpret_cast<const uint4*>(r.ptr + token * r.token + head * r.head);
-    lo = src[c];
-    hi = src[c + 8];
+    lo = __ldcs(src + c);                           // read once
+    hi = __ldcs(src + c + 8);
 }
 __device__ __forceinline__ void store_piece(const Rows& r, int token, int head, int c, const uint4& lo, const uint4& hi) {
     uint4* dst = reinterpret_cast<uint4*>(r.ptr + token * r.token + head * r.head);
@@ -123,57 +145,49 @@ __device__ __forceinline__ void rotate(Piece& x, const Turn& t) {
     }
 }
 
-// Mean key of a complete page in 8 bits.  Every row of the page has been written and is visible to the block.
-template <bool FP8>
-__device__ void summarise_page(const AppendParams& p, int page, int h) {
-    __shared__ double s_sum[kAppendThreads / 32][kD];                  // by warp
+// Mean key of a complete page in 8 bits.  Every row of the page is visible to the block, at `base` (shared memory or the
+// pool), `stride` bytes apart.
+template <bool FP8, int THREADS>
+__device__ void summarise_page(const AppendParams& p, int page, int h, const uint8_t* base, int64_t stride) {
+    constexpr int kGroups = THREADS / 32;          // a warp adds up two rows at a time, a thread 8 of their values
+    __shared__ double s_sum[kGroups][kD];
     __shared__ float s_max[kD / 32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = tid & 7;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = 1 << p.c.log2_page;
-    const uint8_t* base = p.c.k.ptr + page * p.c.k.page + h * p.c.k.head;
-    double sum[16];
+    base += (tid & 15) * (FP8 ? 8 : 16);
+    double sum[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] = 0.0;
-    for (int r = tid >> 3; r < rows; r += kRowsAtOnce) {
-        float f[16];
-        if (FP8) {
-            // e4m3 codes through f16, exactly; a thread owns values 16 c .. 16 c + 15
-            const uint4 x = __ldcg(reinterpret_cast<const uint4*>(base + r * p.c.k.row) + c);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int i = 0; i < 8; ++i) sum[i] = 0.0;
+#pragma unroll 8
+    for (int r = tid >> 4; r < rows; r += 2 * kGroups) {              // 16 rows or more
+        float f[8];
+        if (FP8) {                                  // e4m3 codes through f16, exactly
+            const uint2 x = *reinterpret_cast<const uint2*>(base + r * stride);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t y = e4m3x2_to_f16x2(w[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t y = e4m3x2_to_f16x2((i < 2 ? x.x : x.y) >> (16 * (i & 1)));
                 const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&y));
                 f[2 * i] = v.x;
                 f[2 * i + 1] = v.y;
             }
         } else {
-            float lo[8], hi[8];
-            unpack8(__ldcg(reinterpret_cast<const uint4*>(base + r * p.c.k.row) + 2 * c), lo);
-            unpack8(__ldcg(reinterpret_cast<const uint4*>(base + r * p.c.k.row) + 2 * c + 1), hi);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f[i] = lo[i];
-                f[8 + i] = hi[i];
-            }
+            unpack8(*reinterpret_cast<const uint4*>(base + r * stride), f);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i] += (double)f[i];
+        for (int i = 0; i < 8; ++i) sum[i] += (double)f[i];
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], 8);
-        sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], 16);
-    }
-    if (lane < 8)
+    for (int i = 0; i < 8; ++i) sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], 16);
+    __syncthreads();                                // the sums of the head before have been read
+    if (lane < 16)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_sum[warp][16 * c + i] = sum[i];
+        for (int i = 0; i < 8; ++i) s_sum[warp][lane * 8 + i] = sum[i];
     __syncthreads();
     float mean = 0.0f;
     if (tid < kD) {
         double x = 0.0;
 #pragma unroll
-        for (int w = 0; w < kAppendThreads / 32; ++w) x += s_sum[w][tid];
+        for (int w = 0; w < kGroups; ++w) x += s_sum[w][tid];
         mean = (float)(x / rows);                                     // rows is a power of two: exact before rounding
         if (FP8) mean = __fmul_rn(mean, p.c.k_scale[h]);
         float big = fabsf(mean);
@@ -194,10 +208,11 @@ __device__ void summarise_page(const AppendParams& p, int page, int h) {
     }
 }
 
-// grid (tasks, Hkv + (query ? Hkv : 0)): a task is one page a sequence writes to; y < Hkv: that KV head's keys and
-// values, else the query heads of group y - Hkv.
-template <bool FP8>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendParams p) {
+// grid (tasks, kv_blocks + blocks of query heads): a task is one page a sequence writes to.
+template <bool FP8, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) paged_append_kernel(const __grid_constant__ AppendParams p) {
+    constexpr int kSlots = THREADS / 8;
+    extern __shared__ __align__(128) uint8_t paged_append_smem[];                // rows of the keys as they are stored
     const int tid = threadIdx.x, lane = tid & 31, c = tid & 7;
     // ---- which sequence and page: every warp walks the sequences 32 at a time, nothing is shared
     Span span{0, 0, 0};
@@ -236,80 +251,132 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     const int lo = max(span.start, first), hi = min(span.end, first + rows);    // positions of this task
     const int token0 = span.token - span.start;                                // token of position x: token0 + x
 
-    if ((int)blockIdx.y >= p.Hkv) {
-        const int h0 = ((int)blockIdx.y - p.Hkv) * p.Hg;
-        for (int pos = lo + (tid >> 3); pos < hi; pos += kRowsAtOnce) {
+    // slots of 8 threads, a row each; where there are fewer rows, several heads go side by side
+    int slot_rows = 1;
+    while (slot_rows < kSlots && slot_rows < hi - lo) slot_rows *= 2;
+    const int slot = tid >> 3;
+    const int slot_row = slot % slot_rows, slot_head = slot / slot_rows, head_step = kSlots / slot_rows;
+    bool beyond = false;                            // a position beyond the rotary tables
+
+    if ((int)blockIdx.y >= p.kv_blocks) {
+        const int h0 = ((int)blockIdx.y - p.kv_blocks) * p.q_heads, h1 = min(h0 + p.q_heads, p.H);
+        for (int pos = lo + slot_row; pos < hi; pos += slot_rows) {
             if (p.cos && pos >= p.rope_rows) {
-                raise_status(p.c, kStatusTooLong);
+                beyond = true;
                 continue;
             }
             Turn turn;
             if (p.cos) turn = load_turn(p, pos, c);
-#pragma unroll 4
-            for (int i = 0; i < p.Hg; ++i) {
-                uint4 a, d;
-                load_piece(p.query, token0 + pos, h0 + i, c, a, d);
-                if (p.cos) {
-                    Piece x;
-                    unpack8(a, x.lo);
-                    unpack8(d, x.hi);
-                    rotate(x, turn);
-                    a = pack8(x.lo);
-                    d = pack8(x.hi);
+            constexpr int kAhead = 4;
+            for (int h = h0 + slot_head; h < h1; h += kAhead * head_step) {
+                uint4 a[kAhead], d[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (h + u * head_step < h1) load_piece(p.query, token0 + pos, h + u * head_step, c, a[u], d[u]);
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (h + u * head_step >= h1) break;
+                    if (p.cos) {
+                        Piece x;
+                        unpack8(a[u], x.lo);
+                        unpack8(d[u], x.hi);
+                        rotate(x, turn);
+                        a[u] = pack8(x.lo);
+                        d[u] = pack8(x.hi);
+                    }
+                    store_piece(p.query_out, token0 + pos, h + u * head_step, c, a[u], d[u]);
                 }
-                store_piece(p.query_out, token0 + pos, h0 + i, c, a, d);
             }
         }
+        if (beyond) raise_status(p.c, kStatusTooLong);
         return;
     }
 
-    const int h = blockIdx.y;
-    int page = -1;
-    if (page_index < p.c.table_width) {
-        page = pool_page(p.c, b, page_index);
-        if (page < 0 && tid == 0) raise_status(p.c, kStatusBadPage);
-    } else if (tid == 0) {
-        raise_status(p.c, kStatusTooLong);
-    }
-    const float ks = FP8 ? p.c.k_scale[h] : 1.0f, vs = FP8 ? p.c.v_scale[h] : 1.0f;
-    for (int pos = lo + (tid >> 3); pos < hi; pos += kRowsAtOnce) {
+    const int h0 = blockIdx.y * p.kv_heads, h1 = min(h0 + p.kv_heads, p.Hkv);
+    const bool in_table = page_index < p.c.table_width;
+    const int page = in_table ? pool_page(p.c, b, page_index) : -1;
+    // the page fills up: its mean is wanted, from shared memory where it fits
+    const bool fills = p.codes && page >= 0 && hi == first + rows && (!p.cos || hi <= p.rope_rows);
+    const bool staged = fills && p.staged;
+    constexpr int kRowBytes8 = FP8 ? 128 : 256;
+    if (staged)                                     // rows of earlier calls
+        for (int i = tid; i < (lo - first) * (h1 - h0) * (kRowBytes8 / 16); i += THREADS) {
+            const int at = i / (kRowBytes8 / 16), piece = i % (kRowBytes8 / 16), row = at % (lo - first), h = at / (lo - first);
+            reinterpret_cast<uint4*>(paged_append_smem + (h * rows + row) * kRowBytes8)[piece] =
+                reinterpret_cast<const uint4*>(p.c.k.ptr + page * p.c.k.page + (h0 + h) * p.c.k.head + row * p.c.k.row)[piece];
+        }
+    for (int pos = lo + slot_row; pos < hi; pos += slot_rows) {
         if (p.cos && pos >= p.rope_rows) {
-            raise_status(p.c, kStatusTooLong);
+            beyond = true;
             continue;
         }
-        uint4 ka, kd, va, vd;
-        load_piece(p.key, token0 + pos, h, c, ka, kd);
-        load_piece(p.value, token0 + pos, h, c, va, vd);
-        Piece k;
-        unpack8(ka, k.lo);
-        unpack8(kd, k.hi);
-        if (p.cos) {
-            rotate(k, load_turn(p, pos, c));
-            ka = pack8(k.lo);
-            kd = pack8(k.hi);
-        }
-        if (p.key_out.ptr) store_piece(p.key_out, token0 + pos, h, c, ka, kd);
-        if (page < 0) continue;
-        uint8_t* k_row = p.c.k.ptr + page * p.c.k.page + h * p.c.k.head + (pos - first) * p.c.k.row;
-        uint8_t* v_row = p.c.v.ptr + page * p.c.v.page + h * p.c.v.head + (pos - first) * p.c.v.row;
-        if (FP8) {
-            Piece v;
-            unpack8(va, v.lo);
-            unpack8(vd, v.hi);
-            reinterpret_cast<uint2*>(k_row)[c] = pack8_e4m3(k.lo, ks);
-            reinterpret_cast<uint2*>(k_row)[c + 8] = pack8_e4m3(k.hi, ks);
-            reinterpret_cast<uint2*>(v_row)[c] = pack8_e4m3(v.lo, vs);
-            reinterpret_cast<uint2*>(v_row)[c + 8] = pack8_e4m3(v.hi, vs);
-        } else {
-            reinterpret_cast<uint4*>(k_row)[c] = ka;
-            reinterpret_cast<uint4*>(k_row)[c + 8] = kd;
-            reinterpret_cast<uint4*>(v_row)[c] = va;
-            reinterpret_cast<uint4*>(v_row)[c + 8] = vd;
+        Turn turn;
+        if (p.cos) turn = load_turn(p, pos, c);
+        constexpr int kAhead = 2;
+        for (int hb = h0 + slot_head; hb < h1; hb += kAhead * head_step) {
+            uint4 ka[kAhead], kd[kAhead], va[kAhead], vd[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (hb + u * head_step < h1) {
+                    load_piece(p.key, token0 + pos, hb + u * head_step, c, ka[u], kd[u]);
+                    load_piece(p.value, token0 + pos, hb + u * head_step, c, va[u], vd[u]);
+                }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int h = hb + u * head_step;
+                if (h >= h1) break;
+                Piece k;
+                unpack8(ka[u], k.lo);
+                unpack8(kd[u], k.hi);
+                if (p.cos) {
+                    rotate(k, turn);
+                    ka[u] = pack8(k.lo);
+                    kd[u] = pack8(k.hi);
+                }
+                if (p.key_out.ptr) store_piece(p.key_out, token0 + pos, h, c, ka[u], kd[u]);
+                if (page < 0) continue;
+                uint8_t* k_row = p.c.k.ptr + page * p.c.k.page + h * p.c.k.head + (pos - first) * p.c.k.row;
+                uint8_t* v_row = p.c.v.ptr + page * p.c.v.page + h * p.c.v.head + (pos - first) * p.c.v.row;
+                uint8_t* s_row = paged_append_smem + ((h - h0) * rows + pos - first) * kRowBytes8;
+                if (FP8) {
+                    Piece v;
+                    unpack8(va[u], v.lo);
+                    unpack8(vd[u], v.hi);
+                    const Divisor ks = divisor(p.c.k_scale[h]), vs = divisor(p.c.v_scale[h]);
+                    const uint2 lo8 = pack8_e4m3(k.lo, ks), hi8 = pack8_e4m3(k.hi, ks);
+                    reinterpret_cast<uint2*>(k_row)[c] = lo8;
+                    reinterpret_cast<uint2*>(k_row)[c + 8] = hi8;
+                    if (staged) {
+                        reinterpret_cast<uint2*>(s_row)[c] = lo8;
+                        reinterpret_cast<uint2*>(s_row)[c + 8] = hi8;
+                    }
+                    reinterpret_cast<uint2*>(v_row)[c] = pack8_e4m3(v.lo, vs);
+                    reinterpret_cast<uint2*>(v_row)[c + 8] = pack8_e4m3(v.hi, vs);
+                } else {
+                    reinterpret_cast<uint4*>(k_row)[c] = ka[u];
+                    reinterpret_cast<uint4*>(k_row)[c + 8] = kd[u];
+                    if (staged) {
+                        reinterpret_cast<uint4*>(s_row)[c] = ka[u];
+                        reinterpret_cast<uint4*>(s_row)[c + 8] = kd[u];
+                    }
+                    reinterpret_cast<uint4*>(v_row)[c] = va[u];
+                    reinterpret_cast<uint4*>(v_row)[c + 8] = vd[u];
+                }
+            }
         }
     }
-    if (p.codes && page >= 0 && hi == first + rows && (!p.cos || hi <= p.rope_rows)) {
+    if (beyond) raise_status(p.c, kStatusTooLong);
+    if (page < 0) {
+        if (tid == 0) raise_status(p.c, in_table ? kStatusBadPage : kStatusTooLong);
+        return;
+    }
+    if (fills) {
         __syncthreads();                            // the block's own rows are visible to all of it
-        summarise_page<FP8>(p, page, h);
+        for (int h = h0; h < h1; ++h)
+            if (staged)
+                summarise_page<FP8, THREADS>(p, page, h, paged_append_smem + (h - h0) * rows * kRowBytes8, kRowBytes8);
+            else
+                summarise_page<FP8, THREADS>(p, page, h, p.c.k.ptr + page * p.c.k.page + h * p.c.k.head, p.c.k.row);
     }
 }
 

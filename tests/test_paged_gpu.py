@@ -284,6 +284,15 @@ def _check_append(c, r, rotate=True):
             else:
                 tol = 2.0 ** -8 * y.abs() + 2 * loose if name == "k" and rotate else 0 * y
             assert ((stored - y).abs() <= tol).all(), name
+        # the 32-bit formula, step by step, gives the very codes
+        a, b2 = c["key"][x][..., :64].float(), c["key"][x][..., 64:].float()
+        co, si = cos[:, None], sin[:, None]
+        rot = torch.cat([a * co - b2 * si, b2 * co + a * si], -1) if rotate else c["key"][x].float()
+        if fp8:
+            rot, val = ((y / s[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn) for y, s in ((rot, c["ks"]), (c["value"][x].float(), c["vs"])))
+        else:
+            rot, val = rot.bfloat16(), c["value"][x]
+        assert torch.equal(got["k"][where, :, row].float(), rot.float()) and torch.equal(got["v"][where, :, row].float(), val.float())
     rest = ~touched[:, None, :, None].expand_as(k)
     assert torch.equal(got["k"].float()[rest], c["k"].float()[rest]) and torch.equal(got["v"].float()[rest], c["v"].float()[rest])
     if "codes" in got:
@@ -392,6 +401,30 @@ def test_append_bad_pages_and_lengths():
     c["cu"] = torch.tensor([-7, 2 ** 31 - 1, 3], dtype=torch.int32)
     r = _append(c)
     assert torch.equal(r["k"].cpu(), before)
+
+
+def test_append_codes_over_all_magnitudes():
+    """e4m3 codes of values from 2^-126 to 2^126, near and on the ties between codes, for scales of any mantissa and far from
+    1: those of the 32-bit quotient."""
+    g = torch.Generator().manual_seed(1)
+    T, Hkv = 2048, 16
+    scale = torch.cat([torch.tensor([1.0, 0.5, 3e-30, 7e25, 1.9999999, 2.0 ** -60, 2.0 ** 60, 448.0 ** -1]),
+                       0.01 + torch.rand(8, generator=g)])
+    x = torch.randn(T, Hkv, 128, generator=g) * 2.0 ** torch.randint(-12, 10, (T, Hkv, 128), generator=g)
+    ties = (torch.randint(8, 16, (T, Hkv, 64), generator=g) + 0.5) * 2.0 ** torch.randint(-9, 5, (T, Hkv, 64), generator=g)
+    x[..., :64] = ties * (1 + torch.randint(-2, 3, (T, Hkv, 64), generator=g) * 2.0 ** -8)
+    x = (x * scale[:, None]).bfloat16()
+    x[:32] = (torch.randn(32, Hkv, 128, generator=g) * 2.0 ** torch.randint(-126, 126, (32, Hkv, 128), generator=g)).bfloat16()
+    k = torch.zeros(T // 16, Hkv, 16, 128, device="cuda").to(torch.float8_e4m3fn)
+    v = torch.zeros_like(k)
+    table = torch.arange(T // 16, dtype=torch.int32, device="cuda")[None]
+    s = scale.cuda()
+    aa.paged_kv_append(x.cuda(), x.flip(0).cuda(), k, v, table, torch.tensor([T], dtype=torch.int32, device="cuda"),
+                       cu_seqlens=torch.tensor([0, T], dtype=torch.int32, device="cuda"), k_scale=s, v_scale=s)
+    for pool, y in ((k, x), (v, x.flip(0))):
+        want = (y.float() / scale[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        got = pool.cpu().transpose(1, 2).reshape(T, Hkv, 128)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
 
 
 def test_append_non_finite_keys_and_saturation():
