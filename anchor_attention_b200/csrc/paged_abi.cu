@@ -296,15 +296,25 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     if (tasks > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
     // one token a sequence: a block for every KV head, one for all queries; more tokens: see paged_append.cuh
     const bool single = !a->cu_seqlens && p.per_seq == 1;
-    p.kv_heads = single ? 1 : 2;
-    p.q_heads = single ? (a->H < 64 ? a->H : 64) : 8;
+    p.kv_heads = single ? 1 : c.page_size < aa::paged::kStagedRows ? aa::paged::kStagedRows / c.page_size : 1;
+    p.q_heads = single ? (a->H < 64 ? a->H : 64) : 4 * p.kv_heads;
     p.kv_blocks = (int)ceil_div(c.Hkv, p.kv_heads);
-    p.staged = !single && c.page_size <= aa::paged::kStagedPage;
+    p.staged = !single && c.page_size <= aa::paged::kStagedRows;
     const int64_t q_blocks = a->query ? ceil_div(a->H, p.q_heads) : 0;
     if (p.kv_blocks + q_blocks > 65535) return AA_ERR_TOO_LARGE;
     const dim3 grid((unsigned)tasks, (unsigned)(p.kv_blocks + q_blocks));
     const bool fp8 = c.cache_dtype == AA_E4M3;
-    const size_t smem = p.staged && p.codes ? (size_t)p.kv_heads * c.page_size * (fp8 ? 128 : 256) : 0;
+    const size_t smem = p.staged && p.codes ? (size_t)aa::paged::kStagedRows * (fp8 ? 128 : 256) : 0;
+    static thread_local Device dev;
+    rc = current_device(dev, [] {
+        const int most = aa::paged::kStagedRows * 256;
+        const cudaError_t e = cudaFuncSetAttribute(aa::paged::paged_append_kernel<true, aa::paged::kAppendThreads>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        return e != cudaSuccess ? e
+                                : cudaFuncSetAttribute(aa::paged::paged_append_kernel<false, aa::paged::kAppendThreads>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    });
+    if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     constexpr int kMany = aa::paged::kAppendThreads, kOne = aa::paged::kSingleThreads;
     if (single && fp8)

@@ -24,7 +24,7 @@ namespace paged {
 
 constexpr int kAppendThreads = 256;                // for prompts; a single token a sequence takes kSingleThreads
 constexpr int kSingleThreads = 128;
-constexpr int kStagedPage = 64;                     // pages up to this size are added up in shared memory
+constexpr int kStagedRows = 128;                    // rows of keys (over all heads) a block adds up in shared memory
 
 struct Rows {                                       // [tokens, heads, 128] bf16, strides in elements
     __nv_bfloat16* ptr;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
         }
         Turn turn;
         if (p.cos) turn = load_turn(p, pos, c);
-        constexpr int kAhead = 2;
+        constexpr int kAhead = FP8 ? 1 : 2;      // an e4m3 head has its quotients to wait for
         for (int hb = h0 + slot_head; hb < h1; hb += kAhead * head_step) {
             uint4 ka[kAhead], kd[kAhead], va[kAhead], vd[kAhead];
 #pragma unroll
