@@ -7,9 +7,9 @@
 // cut.  The first and the last pages of a sequence are always kept; the rest go by score, ties to the lower
 // page, and come out in ascending order.
 //
-// A cluster of blocks works on one (sequence, KV head).  Its warps score 16 pages at a time with the 8-bit matrix
-// instruction (pages as its 16 rows, 8 query rows as its columns) and leave the scores as ordered 32-bit keys in the
-// first block's shared memory; that block finds the last key that gets in by counting over 11 + 11 + 10 bits and writes the
+// A cluster of blocks works on one (sequence, KV head).  Its warps score 16 pages at a time, four lanes a page, with
+// four-byte dot products (the 8-bit matrix instruction took 34 SM cycles for 16 pages and 32 bytes, a third of a
+// batch's time), and leave the scores as ordered 32-bit keys in the first block's shared memory; that block finds the last key that gets in by counting over 11 + 11 + 10 bits and writes the
 // list.  The scores are a few dependent loads per page, so a small batch is a matter of latency: eight blocks
 // share a sequence there, and each warp has 32 pages' loads in flight.
 #pragma once
@@ -202,22 +202,34 @@ __global__ void __launch_bounds__(kSelectThreads, 4) page_select_kernel(const __
     const uint32_t keys_at = cluster > 1 ? in_first_block(smem_u32(s_key)) : 0;
     auto score = [&](int base, const PageTile& x) {
         float best[2] = {-INFINITY, -INFINITY};
-        const uint32_t a0[4] = {x.lo[0].x, x.lo[1].x, x.lo[0].y, x.lo[1].y};
-        const uint32_t a1[4] = {x.lo[0].z, x.lo[1].z, x.lo[0].w, x.lo[1].w};
-        const uint32_t a2[4] = {x.hi[0].x, x.hi[1].x, x.hi[0].y, x.hi[1].y};
-        const uint32_t a3[4] = {x.hi[0].z, x.hi[1].z, x.hi[0].w, x.hi[1].w};
-        for (int n = 0; n < row_tiles; ++n) {
-            const uint4* q = reinterpret_cast<const uint4*>(s_q + (n * 8 + g) * 32);
-            const uint4 u = q[t], w = q[4 + t];
-            int d[4] = {0, 0, 0, 0};
-            mma_s8(d, a0, u.x, u.y);
-            mma_s8(d, a1, u.z, u.w);
-            mma_s8(d, a2, w.x, w.y);
-            mma_s8(d, a3, w.z, w.w);
+        const uint32_t w0[8] = {x.lo[0].x, x.lo[0].y, x.lo[0].z, x.lo[0].w, x.hi[0].x, x.hi[0].y, x.hi[0].z, x.hi[0].w};
+        const uint32_t w1[8] = {x.lo[1].x, x.lo[1].y, x.lo[1].z, x.lo[1].w, x.hi[1].x, x.hi[1].y, x.hi[1].z, x.hi[1].w};
+#pragma unroll 1
+        for (int r0 = 0; r0 < p.rows; r0 += 4) {
+            int d[2][4];                            // this lane's share of the products of its pages with four rows
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = n * 8 + 2 * t + (i & 1);
-                if (r < p.rows) best[i >> 1] = fmaxf(best[i >> 1], __fmul_rn((float)d[i], s_scale[r]));
+            for (int r = 0; r < 4; ++r) {
+                const uint4* q = reinterpret_cast<const uint4*>(s_q + (r0 + r) * 32);
+                const uint4 u = q[t], v = q[4 + t];
+                const uint32_t c[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                int e0 = 0, e1 = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e0 = __dp4a((int)w0[i], (int)c[i], e0);
+                    e1 = __dp4a((int)w1[i], (int)c[i], e1);
+                }
+                d[0][r] = e0;
+                d[1][r] = e1;
+            }
+            // added up over the four lanes of a page, so that lane t ends with row r0 + t
+            const float row_scale = s_scale[r0 + t];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool up1 = t & 2, up0 = t & 1;
+                const int k0 = (up1 ? d[i][2] : d[i][0]) + __shfl_xor_sync(0xFFFFFFFFu, up1 ? d[i][0] : d[i][2], 2);
+                const int k1 = (up1 ? d[i][3] : d[i][1]) + __shfl_xor_sync(0xFFFFFFFFu, up1 ? d[i][1] : d[i][3], 2);
+                const int all = (up0 ? k1 : k0) + __shfl_xor_sync(0xFFFFFFFFu, up0 ? k0 : k1, 1);
+                if (r0 + t < p.rows) best[i] = fmaxf(best[i], __fmul_rn((float)all, row_scale));
             }
         }
 #pragma unroll

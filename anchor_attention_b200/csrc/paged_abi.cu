@@ -83,6 +83,22 @@ aa::paged::Cache view(const aa_paged_cache_t& c, int log2_page) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Launches a kernel that starts with griddepcontrol.wait: its launch overlaps the end of the kernel before it on the stream.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- tensor maps: a pool [pages, Hkv, page_size, 128] as a 4-D map, dimension 0 the row, the others by increasing
 // stride (a dimension of size 1 last, where its stride does not matter).  A copy takes 128 bytes of `box` rows.
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -201,17 +217,8 @@ int launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const aa::
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_attend");
     if (!pl.split) return AA_OK;
-    // the join kernel's launch overlaps the attention kernel's end; it waits on the device for its results
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pl.ctas - 1, 8 * RW < pl.rows ? 8 * RW : pl.rows);
-    cfg.blockDim = dim3(aa::paged::kJoinThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, aa::paged::paged_join_kernel<FP8>, p, 8 * RW);
+    e = launch_after(aa::paged::paged_join_kernel<FP8>, dim3(pl.ctas - 1, 8 * RW < pl.rows ? 8 * RW : pl.rows),
+                     dim3(aa::paged::kJoinThreads), 0, st, p, 8 * RW);
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_join");
     return AA_OK;
 }

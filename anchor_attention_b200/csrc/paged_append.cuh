@@ -86,22 +86,6 @@ __device__ __forceinline__ void unpack8(const uint4& x, float (&f)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
-// Division by one number for many: q = x r with r = 1 / s rounded, then one step q + (x - q s) r.  The step gives the
-// correctly rounded quotient (P. Markstein, Computation of elementary functions on the IBM RISC System/6000
-// processor, 1990) as long as nothing overflows or vanishes; what is not in a safe range divides.
-struct Divisor {
-    float s, r;
-    bool plain;                                     // s in a range where r and the step's products are normal numbers
-};
-__device__ __forceinline__ Divisor divisor(float s) {
-    return Divisor{s, __fdiv_rn(1.0f, s), s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7FFFFFu) != 0x7FFFFFu};
-}
-__device__ __forceinline__ float divide(float x, const Divisor& d) {
-    // below 2^-60 / 2^60 the quotient's code is 0 whatever its last bit, above (or not finite) it saturates or is NaN
-    if (!d.plain || !(fabsf(x) <= 0x1p60f)) return __fdiv_rn(x, d.s);
-    const float q = __fmul_rn(x, d.r);
-    return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
-}
 __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], const Divisor& d) {
     uint32_t w[2] = {0, 0};
 #pragma unroll

@@ -52,6 +52,26 @@ __device__ __forceinline__ int pool_page(const Cache& c, int b, int logical) {
     return (uint32_t)p < (uint32_t)c.pages ? p : -1;
 }
 
+// ---- quotients
+// Division by one number for many: q = x r with r = 1 / s rounded, then one step q + (x - q s) r.  The step gives the
+// correctly rounded quotient (P. Markstein, Computation of elementary functions on the IBM RISC System/6000
+// processor, 1990) as long as nothing overflows or vanishes; what is not in a safe range divides.
+struct Divisor {
+    float s, r;
+    bool plain;                                     // s in a range where r and the step's products are normal numbers
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+    return Divisor{s, __fdiv_rn(1.0f, s), s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7FFFFFu) != 0x7FFFFFu};
+}
+__device__ __forceinline__ float quotient(float x, const Divisor& d) {              // d.plain, |x| up to 2^60
+    const float q = __fmul_rn(x, d.r);
+    return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
+}
+__device__ __forceinline__ float divide(float x, const Divisor& d) {
+    // a quotient so small that the step's remainder vanishes has the code 0 whatever its last bit
+    return d.plain && fabsf(x) <= 0x1p60f ? quotient(x, d) : __fdiv_rn(x, d.s);
+}
+
 // ---- matrix instructions of one warp ---------------------------------------------------------------------
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
