@@ -121,6 +121,8 @@ __global__ void __launch_bounds__(kSelectThreads, 4) page_select_kernel(const __
     uint32_t* s_q = reinterpret_cast<uint32_t*>(s_hist + kBins);                  // [padded][32] four codes each
     float* s_scale = reinterpret_cast<float*>(s_q + padded * 32);                 // [padded]
 
+    start_next_kernel();
+    wait_for_kernels_before();
     const int len = seq_len(p.c, b);
     if (tid == 0 && h == 0 && rank == 0 && p.c.seq_lens[b] > ((int64_t)p.c.table_width << p.c.log2_page))
         raise_status(p.c, kStatusTooLong);
@@ -198,7 +200,6 @@ __global__ void __launch_bounds__(kSelectThreads, 4) page_select_kernel(const __
     if (cluster > 1) cluster_wait();
 
     // ---- scores
-    const int row_tiles = padded / 8;
     const uint32_t keys_at = cluster > 1 ? in_first_block(smem_u32(s_key)) : 0;
     auto score = [&](int base, const PageTile& x) {
         float best[2] = {-INFINITY, -INFINITY};

@@ -83,19 +83,23 @@ aa::paged::Cache view(const aa_paged_cache_t& c, int log2_page) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Launches a kernel that starts with griddepcontrol.wait: its launch overlaps the end of the kernel before it on the stream.
+// Launches a kernel that waits for those before it on the device (wait_for_kernels_before): the launch itself and the
+// kernel's start overlap their end.
 template <typename... P, typename... A>
-cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -199,7 +203,7 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
     if (entries * units > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
     const int64_t most = (int64_t)dev.sms * aa::paged::kCtasPerSm;
     pl.ctas = (int)(entries * units < most ? entries * units : most);
-    if (pl.ctas > 512) pl.ctas = 512;             // the join kernel's table of weights
+    if (pl.ctas > 512) pl.ctas = 512;             // the kernel's 32-bit ranges
     pl.split = units > 1 && pl.ctas > 1;
     const size_t parts = pl.split ? (size_t)pl.ctas * 2 * 8 * pl.tiles8 : 0;
     pl.o_off = 0;
@@ -212,13 +216,12 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
 template <bool FP8, int RW>
 int launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const aa::paged::AttendParams& p, const AttendPlan& pl,
                   cudaStream_t st) {
-    aa::paged::paged_attend_kernel<FP8, RW>
-        <<<pl.ctas, aa::paged::Shape<FP8, RW>::kThreads, aa::paged::kSmemBytes, st>>>(k_map, v_map, p);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e = launch_after(aa::paged::paged_attend_kernel<FP8, RW>, dim3(pl.ctas), dim3(aa::paged::Shape<FP8, RW>::kThreads),
+                                 aa::paged::kSmemBytes, st, 1, k_map, v_map, p);
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_attend");
     if (!pl.split) return AA_OK;
     e = launch_after(aa::paged::paged_join_kernel<FP8>, dim3(pl.ctas - 1, 8 * RW < pl.rows ? 8 * RW : pl.rows),
-                     dim3(aa::paged::kJoinThreads), 0, st, p, 8 * RW);
+                     dim3(aa::paged::kJoinThreads), 0, st, 1, p, 8 * RW);
     if (e != cudaSuccess) return record_cuda_error(e, "launch paged_join");
     return AA_OK;
 }
@@ -324,15 +327,15 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     constexpr int kMany = aa::paged::kAppendThreads, kOne = aa::paged::kSingleThreads;
+    cudaError_t e;
     if (single && fp8)
-        aa::paged::paged_append_kernel<true, kOne><<<grid, kOne, 0, st>>>(p);
+        e = launch_after(aa::paged::paged_append_kernel<true, kOne>, grid, dim3(kOne), 0, st, 1, p);
     else if (single)
-        aa::paged::paged_append_kernel<false, kOne><<<grid, kOne, 0, st>>>(p);
+        e = launch_after(aa::paged::paged_append_kernel<false, kOne>, grid, dim3(kOne), 0, st, 1, p);
     else if (fp8)
-        aa::paged::paged_append_kernel<true, kMany><<<grid, kMany, smem, st>>>(p);
+        e = launch_after(aa::paged::paged_append_kernel<true, kMany>, grid, dim3(kMany), smem, st, 1, p);
     else
-        aa::paged::paged_append_kernel<false, kMany><<<grid, kMany, smem, st>>>(p);
-    cudaError_t e = cudaGetLastError();
+        e = launch_after(aa::paged::paged_append_kernel<false, kMany>, grid, dim3(kMany), smem, st, 1, p);
     return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch paged_append");
 }
 
@@ -428,18 +431,8 @@ int aa_page_select(const aa_page_select_t* a, void* stream) {
     while (cluster < aa::paged::kMaxSelectCluster && (int64_t)c.B * c.Hkv * cluster < 2 * dev.sms &&
            c.table_width > cluster * aa::paged::kSelectWarps * 16)
         cluster *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(c.B * c.Hkv * cluster));
-    cfg.blockDim = dim3(aa::paged::kSelectThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, aa::paged::page_select_kernel, p, cluster);
+    const cudaError_t e = launch_after(aa::paged::page_select_kernel, dim3((unsigned)(c.B * c.Hkv * cluster)),
+                                       dim3(aa::paged::kSelectThreads), smem, static_cast<cudaStream_t>(stream), cluster, p, cluster);
     return e == cudaSuccess ? AA_OK : record_cuda_error(e, "launch page_select");
 }
 

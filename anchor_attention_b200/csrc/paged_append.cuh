@@ -198,6 +198,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
     constexpr int kSlots = THREADS / 8;
     extern __shared__ __align__(128) uint8_t paged_append_smem[];                // rows of the keys as they are stored
     const int tid = threadIdx.x, lane = tid & 31, c = tid & 7;
+    start_next_kernel();
+    wait_for_kernels_before();
     // ---- which sequence and page: every warp walks the sequences 32 at a time, nothing is shared
     Span span{0, 0, 0};
     int b = 0, page_index = -1;

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     static_assert(16 * kStages + kSegments * 8 + (S::kLanes * kStages + S::kWarps + 4) * 4 <= kMiscBytes, "the last 512 bytes");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    start_next_kernel();
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
             tc::mbar_init(full(i), 1);
@@ -303,7 +303,10 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
         }
         *abort_flag = 0;
         tc::fence_mbar_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
     }
+    wait_for_kernels_before();
 
     // ---- this CTA's range of the line of units
     const int entries = p.B * p.Hkv * p.row_tiles;
@@ -330,8 +333,10 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
         if (tid == 0) p.cuts[blockIdx.x] = make_int2(-1, 0);
         return;
     }
-    const int begin = (int)((int64_t)total * blockIdx.x / ctas);
-    const int end = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
+    // CTA c owns the units [total c / ctas, total (c + 1) / ctas), in 32-bit arithmetic (ctas is at most 512)
+    const int whole_part = total / ctas, rest = total - whole_part * ctas;
+    auto range_start = [&](int c) { return whole_part * c + rest * c / ctas; };
+    const int begin = range_start(blockIdx.x), end = range_start(blockIdx.x + 1);
     if (begin >= before && begin < before + mine) {
         int e = my_first, at = before;
         for (int n = entry_units(p, e, S::kUnitKeys); at + n <= begin; n = entry_units(p, e, S::kUnitKeys)) {
@@ -361,11 +366,14 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     enter(p, now, first_entry, S::kUnitKeys, segments, first_entry);
     now.unit = first_unit;
     if (tid == 0) {
-        // CTA c owns the units [total c / ctas, total (c + 1) / ctas), so unit u belongs to CTA ((u + 1) ctas - 1) / total
         const int starts = begin - first_unit;
-        const bool leads = first_unit > 0 && (int)((int64_t)total * (blockIdx.x - 1) / ctas) <= starts;
-        const int last = (int)(((int64_t)(starts + now.units) * ctas - 1) / total);
-        p.cuts[blockIdx.x] = leads ? make_int2(first_entry, last - (int)blockIdx.x + 2) : make_int2(-1, 0);
+        int2 cut = make_int2(-1, 0);
+        if (first_unit > 0 && range_start(blockIdx.x - 1) <= starts) {
+            // unit u belongs to CTA ((u + 1) ctas - 1) / total: 40 bits by 31, exact in double precision
+            const int last = (int)(((double)(starts + now.units) * ctas - 1.0) / total);
+            cut = make_int2(first_entry, last - (int)blockIdx.x + 2);
+        }
+        p.cuts[blockIdx.x] = cut;
     }
 
     if (warp == S::kWarps) {
@@ -629,16 +637,17 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
 
 // Adds up the parts of the entries that a cut of the line went through.  Block (c - 1, r) takes row r of the entry that CTA
 // c leads (see `cuts`): CTA c - 1 began it, c, c + 1, ... start inside it.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 128;
 
 template <bool FP8>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ AttendParams p, int tile_rows) {
-    __shared__ float s_weight[512];
-    __shared__ float s_red[kJoinThreads / 32];
-    __shared__ float4 s_acc[kJoinThreads / 32][32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kWarps = kJoinThreads / 32, kAhead = 4;
+    __shared__ float s_sum[kWarps];
+    __shared__ float4 s_acc[kWarps][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x + 1, rr = blockIdx.y;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_next_kernel();
+    wait_for_kernels_before();
     const int2 cut = p.cuts[c];
     const int entry = cut.x, parts = cut.y;         // parts i = 0 .. parts - 1 come from CTAs c - 1 + i
     if (entry < 0) return;
@@ -647,46 +656,44 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     if (r >= p.rows) return;
     auto index = [&](int i) { return ((int64_t)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * tile_rows + rr; };
 
+    // warp w takes parts w, w + 8, ...; the first are on their way while every warp finds the maximum of all
+    float4 x[kAhead];
+    float2 ml[kAhead];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i0 + u * kWarps < parts) {
+                ml[u] = p.part_ml[index(i0 + u * kWarps)];
+                x[u] = reinterpret_cast<const float4*>(p.part_o + index(i0 + u * kWarps) * kD)[lane];
+            }
+    };
+    fetch(warp);
     float top = -INFINITY;
-    for (int i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, p.part_ml[index(i)].x);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[index(i)].x);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    if (lane == 0) s_red[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[w]);
-    __syncthreads();
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
-    for (int i = tid; i < parts; i += kJoinThreads) {
-        const float2 ml = p.part_ml[index(i)];
-        const float f = fast_exp2(ml.x - ref);
-        s_weight[i] = f;
-        sum += f * ml.y;
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    if (lane == 0) s_red[warp] = sum;
-    __syncthreads();
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[w];
-
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = warp; i < parts; i += kJoinThreads / 32) {
-        const float4 x = reinterpret_cast<const float4*>(p.part_o + index(i) * kD)[lane];
-        const float f = s_weight[i];
-        acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    for (int i0 = warp; i0 < parts; i0 += kAhead * kWarps) {
+        if (i0 > warp) fetch(i0);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i0 + u * kWarps >= parts) break;
+            const float f = fast_exp2(ml[u].x - ref);
+            sum += f * ml[u].y;
+            acc.x += f * x[u].x; acc.y += f * x[u].y; acc.z += f * x[u].z; acc.w += f * x[u].w;
+        }
     }
     s_acc[warp][lane] = acc;
+    if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-        acc = s_acc[0][lane];
 #pragma unroll
-        for (int w = 1; w < kJoinThreads / 32; ++w) {
-            const float4 x = s_acc[w][lane];
-            acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+        for (int w = 1; w < kWarps; ++w) {
+            const float4 y = s_acc[w][lane];
+            acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+            sum += s_sum[w];
         }
         const int bh = entry / p.row_tiles, b = bh / p.Hkv, h = bh - b * p.Hkv;
         const int j = r / p.Hg, head = h * p.Hg + (r - j * p.Hg);

@@ -20,6 +20,12 @@ constexpr uint32_t kStatusTimeout = 4;   // a bounded wait gave up
 // An 8-bit code's scale is the largest magnitude times this: the product, not a division, is the definition.
 constexpr float kInv127 = 1.0f / 127.0f;
 
+// Every kernel here starts in the shadow of the one before it on the stream and lets the next do the same
+// (programmatic launch): nothing in global memory is touched before wait_for_kernels_before(), which returns when all earlier
+// kernels are done and their writes visible.
+__device__ __forceinline__ void start_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_kernels_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Pool {
     uint8_t* ptr;
     int64_t page, head, row;             // strides in bytes
