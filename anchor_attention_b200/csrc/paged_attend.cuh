@@ -34,7 +34,7 @@
 namespace aa {
 namespace paged {
 
-constexpr int kTileKeys = 16;                       // keys of one lane and step
+constexpr int kTileKeys = 16;                       // keys of one matrix instruction
 constexpr int kCombStride = 132;                    // floats; 132 keeps the transposed writes off each other's banks
 constexpr int kCombRows = 32;                       // rows of partial results a round of adding up holds
 constexpr int kCombBytes = kCombRows * kCombStride * 4;
@@ -44,13 +44,19 @@ constexpr int kSegments = 16;                       // entries of a CTA's range 
 constexpr int kMiscBytes = 512;
 constexpr int kSmemBytes = kRingBytes + kCombBytes + kMiscBytes;
 
-// The warps of a CTA (and one more, the producer) and the stages of its ring.
+// The warps of a CTA (and one more, the producer) and the stages of its ring.  Four computing warps where it can be: two CTAs
+// then leave each thread 162 registers, and a warp that takes two or four tiles of 16 keys a step has enough of its own to
+// hide its latencies.  Measured at 32 sequences of up to 32768 tokens, e4m3, a group of 4: 8 lanes of one tile 196 us, 4 of
+// two 188 us; eight sequences of up to 16001 tokens, bf16: 20 rows 85 us with one tile, 74 us with two, 32 rows 99 us with 2 lanes
+// of two tiles, 87 us with one of four, 12 rows 76 us with 4 lanes of one, 66 us with 2 of two; e4m3, 12 rows: 63 and 53 us.
 template <bool FP8, int RW>
 struct Shape {
-    static constexpr int kLanes = RW == 1 ? (FP8 ? 8 : 4) : RW == 2 ? 4 : 2;
+    static constexpr int kLanes = RW == 1 ? 4 : RW < 4 ? 2 : 1;
+    static constexpr int kDepth = RW == 1 ? (FP8 ? 2 : 1) : FP8 || RW == 4 ? 4 : 2;     // tiles of a lane and step
+    static constexpr int kTiles = kLanes * kDepth;                                      // of a unit
     static constexpr int kWarps = kLanes * RW;
     static constexpr int kThreads = (kWarps + 1) * 32;
-    static constexpr int kUnitKeys = kLanes * kTileKeys;
+    static constexpr int kUnitKeys = kTiles * kTileKeys;
     static constexpr int kParts = FP8 ? 2 : 4;                       // of 128 bytes a key: keys, values, or halves of them
     static constexpr int kPartBytes = kUnitKeys * 128;
     static constexpr int kUnitBytes = kParts * kPartBytes;
@@ -119,9 +125,9 @@ __device__ __forceinline__ void enter(const AttendParams& p, Cursor& c, int entr
     }
 }
 
-// Where the 16 keys of (cursor, lane) are: the pool page, or -1 for none; `pos` their first position.
-__device__ __forceinline__ int locate(const AttendParams& p, const Cursor& c, int lanes, int lane, int& pos) {
-    const int64_t flat = ((int64_t)c.unit * lanes + lane) * kTileKeys;
+// Where the 16 keys of a tile of the cursor's unit are: the pool page, or -1 for none; `pos` their first position.
+__device__ __forceinline__ int locate(const AttendParams& p, const Cursor& c, int tiles, int tile, int& pos) {
+    const int64_t flat = ((int64_t)c.unit * tiles + tile) * kTileKeys;
     int logical = (int)(flat >> p.c.log2_page);
     const int within = (int)(flat & ((1 << p.c.log2_page) - 1));
     if (p.pages) {
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                         const __grid_constant__ AttendParams p) {
     using S = Shape<FP8, RW>;
-    constexpr int kStages = S::kStages;
+    constexpr int kStages = S::kStages, kDepth = S::kDepth;
     extern __shared__ __align__(1024) uint8_t paged_attend_smem[];
     float* comb = reinterpret_cast<float*>(paged_attend_smem + kRingBytes);
     // the last 512 bytes: barriers, lengths of this range's entries, tile positions of the stages, scratch of the start
@@ -289,10 +295,10 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     auto full = [&](uint32_t stage) { return bars + 8u * stage; };
     auto empty = [&](uint32_t stage) { return bars + 8u * (kStages + stage); };
     int2* segments = reinterpret_cast<int2*>(paged_attend_smem + kRingBytes + kCombBytes + 16 * kStages);
-    int* s_pos = reinterpret_cast<int*>(segments + kSegments);                    // [stages][lanes], -1: no keys
-    int* s_sum = s_pos + S::kLanes * kStages;                                     // [warps], then (entry, unit)
+    int* s_pos = reinterpret_cast<int*>(segments + kSegments);                    // [stages][tiles], -1: no keys
+    int* s_sum = s_pos + S::kTiles * kStages;                                     // [warps], then (entry, unit)
     volatile int* abort_flag = s_sum + S::kWarps + 3;
-    static_assert(16 * kStages + kSegments * 8 + (S::kLanes * kStages + S::kWarps + 4) * 4 <= kMiscBytes, "the last 512 bytes");
+    static_assert(16 * kStages + kSegments * 8 + (S::kTiles * kStages + S::kWarps + 4) * 4 <= kMiscBytes, "the last 512 bytes");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     start_next_kernel();
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
 
     if (warp == S::kWarps) {
         // ================================================== producer
-        // lane i < kLanes looks up tile i of the unit; lane 8 * part + box issues a copy
+        // lane i < kTiles looks up tile i of the unit; lane 8 * part + box issues a copy
         const int boxes = S::kUnitKeys >> p.log2_box, box_bytes = 128 << p.log2_box;
         const int box = lane & 7, part = lane >> 3;
         const bool issues = part < S::kParts && box < boxes;
@@ -387,7 +393,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
         const MapOrder order = of_values ? p.v_order : p.k_order;
         const int x = FP8 ? 0 : (part & 1) * 64;
         const uint32_t box_at = part * S::kPartBytes + box * box_bytes;
-        int pos = 0, page = lane < S::kLanes ? locate(p, now, S::kLanes, lane, pos) : -1;
+        int pos = 0, page = lane < S::kTiles ? locate(p, now, S::kTiles, lane, pos) : -1;
         uint32_t stage = 0, parity = 1;             // of the stage's previous use: the first pass waits for nothing
         for (int i = 0; i < left; ++i) {
             tc::mbar_wait(empty(stage), parity, abort_flag);
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
             const int box_pos = __shfl_sync(0xFFFFFFFFu, pos, first_tile & 31);
             const bool issue = issues && box_page >= 0;
             const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, issue)) * box_bytes;
-            if (lane < S::kLanes) s_pos[stage * S::kLanes + lane] = page >= 0 ? pos : -1;
+            if (lane < S::kTiles) s_pos[stage * S::kTiles + lane] = page >= 0 ? pos : -1;
             __syncwarp();
             if (lane == 0) tc::mbar_arrive_expect_tx(full(stage), bytes);
             __syncwarp();
@@ -414,7 +420,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                     enter(p, now, now.entry + 1, S::kUnitKeys, segments, first_entry);
                     now.unit = 0;
                 }
-                page = lane < S::kLanes ? locate(p, now, S::kLanes, lane, pos) : -1;   // used after the next wait
+                page = lane < S::kTiles ? locate(p, now, S::kTiles, lane, pos) : -1;   // used after the next wait
             }
             if (++stage == kStages) {
                 stage = 0;
@@ -463,51 +469,66 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
         for (int step = 0; step < todo; ++step) {
             const uint32_t free_bar = empty(stage);
             const bool landed = tc::mbar_wait(full(stage), parity, abort_flag);
-            const int pos = landed ? s_pos[stage * S::kLanes + kl] : -1;
-            const uint32_t slot = ring + stage * S::kUnitBytes + kl * (kTileKeys * 128);
+            int pos[kDepth];
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j) {
+                pos[j] = landed ? s_pos[stage * S::kTiles + kl * kDepth + j] : -1;
+                any = any || pos[j] >= 0;
+            }
+            const uint32_t slot0 = ring + stage * S::kUnitBytes + kl * kDepth * (kTileKeys * 128);
             if (++stage == kStages) {
                 stage = 0;
                 parity ^= 1;
             }
-            if (__any_sync(0xFFFFFFFFu, pos < 0)) {
+            if (!__all_sync(0xFFFFFFFFu, any)) {
                 if (lane == 0) tc::mbar_arrive(free_bar);
                 continue;
             }
-            // ---- scores, in two sums: s = keys (g, g, g+8, g+8) x rows (2t, 2t+1, 2t, 2t+1)
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (!FP8) {
+            // ---- scores, in two sums a tile: s = keys (g, g, g+8, g+8) x rows (2t, 2t+1, 2t, 2t+1)
+            float s[kDepth][4];
+            bool edge = false;                      // some row does not see all keys
 #pragma unroll
-                for (int ks = 0; ks < 8; ks += 2) {
-                    uint32_t a[4], a2[4];
-                    ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + (lane >> 4)), a);
-                    ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + 2 + (lane >> 4)), a2);
-                    mma_bf16(s, a, qf.f[ks][0], qf.f[ks][1]);
-                    mma_bf16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
+            for (int j = 0; j < kDepth; ++j) {
+                const uint32_t slot = slot0 + j * (kTileKeys * 128);
+                float s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (!FP8) {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks += 2) {
+                        uint32_t a[4], a2[4];
+                        ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + (lane >> 4)), a);
+                        ldmatrix4(tile_addr<false, RW>(slot, lane & 15, 2 * ks + 2 + (lane >> 4)), a2);
+                        mma_bf16(s1, a, qf.f[ks][0], qf.f[ks][1]);
+                        mma_bf16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks += 2) {
+                        uint32_t x[4];
+                        ldmatrix4(tile_addr<true, RW>(slot, lane & 15, ks + (lane >> 4)), x);
+                        const uint32_t a[4] = {e4m3x2_to_f16x2(x[0]), e4m3x2_to_f16x2(x[1]), e4m3x2_to_f16x2(x[0] >> 16),
+                                               e4m3x2_to_f16x2(x[1] >> 16)};
+                        const uint32_t a2[4] = {e4m3x2_to_f16x2(x[2]), e4m3x2_to_f16x2(x[3]), e4m3x2_to_f16x2(x[2] >> 16),
+                                                e4m3x2_to_f16x2(x[3] >> 16)};
+                        mma_f16(s1, a, qf.f[ks][0], qf.f[ks][1]);
+                        mma_f16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
+                    }
                 }
-            } else {
+                const bool cut_off = pos[j] < 0 || pos[j] + kTileKeys > all_see;
+                edge = edge || cut_off;
 #pragma unroll
-                for (int ks = 0; ks < 8; ks += 2) {
-                    uint32_t x[4];
-                    ldmatrix4(tile_addr<true, RW>(slot, lane & 15, ks + (lane >> 4)), x);
-                    const uint32_t a[4] = {e4m3x2_to_f16x2(x[0]), e4m3x2_to_f16x2(x[1]), e4m3x2_to_f16x2(x[0] >> 16),
-                                           e4m3x2_to_f16x2(x[1] >> 16)};
-                    const uint32_t a2[4] = {e4m3x2_to_f16x2(x[2]), e4m3x2_to_f16x2(x[3]), e4m3x2_to_f16x2(x[2] >> 16),
-                                            e4m3x2_to_f16x2(x[3] >> 16)};
-                    mma_f16(s, a, qf.f[ks][0], qf.f[ks][1]);
-                    mma_f16(s2, a2, qf.f[ks + 1][0], qf.f[ks + 1][1]);
+                for (int x = 0; x < 4; ++x) {
+                    s[j][x] = (s1[x] + s2[x]) * scale[x & 1];
+                    if (cut_off && (pos[j] < 0 || pos[j] + g + (x >> 1) * 8 >= limit[x & 1])) s[j][x] = -INFINITY;
                 }
             }
             // ---- softmax step
-            const bool edge = pos + kTileKeys > all_see;
             float corr[2];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                s[x] = (s[x] + s2[x]) * scale[x & 1];
-                if (edge && pos + g + (x >> 1) * 8 >= limit[x & 1]) s[x] = -INFINITY;
-            }
-#pragma unroll
             for (int x = 0; x < 2; ++x) {
-                float top = fmaxf(s[x], s[x + 2]);
+                float top = fmaxf(s[0][x], s[0][x + 2]);
+#pragma unroll
+                for (int j = 1; j < kDepth; ++j) top = fmaxf(top, fmaxf(s[j][x], s[j][x + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
@@ -515,9 +536,14 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 const float ref = m_new == -INFINITY ? 0.0f : m_new;       // a row that has seen nothing yet
                 corr[x] = fast_exp2(m[x] - ref);
                 m[x] = m_new;
-                s[x] = fast_exp2(s[x] - ref);
-                s[x + 2] = fast_exp2(s[x + 2] - ref);
-                l[x] = l[x] * corr[x] + (s[x] + s[x + 2]);
+                float more = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kDepth; ++j) {
+                    s[j][x] = fast_exp2(s[j][x] - ref);
+                    s[j][x + 2] = fast_exp2(s[j][x + 2] - ref);
+                    more += s[j][x] + s[j][x + 2];
+                }
+                l[x] = l[x] * corr[x] + more;
             }
             if (__any_sync(0xFFFFFFFFu, corr[0] != 1.0f || corr[1] != 1.0f)) {
 #pragma unroll
@@ -525,41 +551,44 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) o[i][x] *= corr[x & 1];
             }
-            uint32_t ph[2], pl[2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const float a = s[2 * half], b = s[2 * half + 1];
-                if (FP8) {
-                    ph[half] = movmatrix_trans(pack_f16x2(a, b));
-                    pl[half] = 0;
-                } else {
-                    // the upper 8 bits, and the rest -- a hair more of it, so that a probability above
-                    // zero has two parts above zero and an infinite value stays infinite, not NaN
-                    const uint32_t hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-                    const float more = 1.0f + 0x1p-23f;
-                    ph[half] = movmatrix_trans(hi);
-                    pl[half] = movmatrix_trans(pack_bf16x2(fmaf(a, more, -__uint_as_float(hi << 16)),
-                                                           fmaf(b, more, -__uint_as_float(hi & 0xFFFF0000u))));
+            for (int j = 0; j < kDepth; ++j) {
+                uint32_t ph[2], pl[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float a = s[j][2 * half], b = s[j][2 * half + 1];
+                    if (FP8) {
+                        ph[half] = movmatrix_trans(pack_f16x2(a, b));
+                        pl[half] = 0;
+                    } else {
+                        // the upper 8 bits, and the rest -- a hair more of it, so that a probability above
+                        // zero has two parts above zero and an infinite value stays infinite, not NaN
+                        const uint32_t hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+                        const float more = 1.0f + 0x1p-23f;
+                        ph[half] = movmatrix_trans(hi);
+                        pl[half] = movmatrix_trans(pack_bf16x2(fmaf(a, more, -__uint_as_float(hi << 16)),
+                                                               fmaf(b, more, -__uint_as_float(hi & 0xFFFF0000u))));
+                    }
                 }
-            }
-            const uint32_t v_slot = slot + S::kUnitBytes / 2;
-            bool own[2] = {false, false};
-            if (!edge) {
-                value_product<FP8, RW, false>(v_slot, lane, ph, pl, o, 0, 0, own);
-            } else {
-                // Keys behind the end, or that only some of the rows may see: a masked probability of zero does not
-                // protect a row from an infinity or NaN in a value, so every new token gets a product of its own
-                // with the values behind its position cleared (one or two tiles of an entry).
-                const int j1 = (min(row0 + 8, p.rows) - 1) / p.Hg;
+                const uint32_t v_slot = slot0 + j * (kTileKeys * 128) + S::kUnitBytes / 2;
+                bool own[2] = {false, false};
+                if (!edge) {
+                    value_product<FP8, RW, false>(v_slot, lane, ph, pl, o, 0, 0, own);
+                } else if (pos[j] >= 0) {
+                    // Keys behind the end, or that only some of the rows may see: a masked probability of zero does not
+                    // protect a row from an infinity or NaN in a value, so every new token gets a product of its own
+                    // with the values behind its position cleared (one or two tiles of an entry).
+                    const int j1 = (min(row0 + 8, p.rows) - 1) / p.Hg;
 #pragma unroll 1
-                for (int j = row0 / p.Hg; j <= j1; ++j) {
-                    const int seen = all_see + j - pos;                         // keys of the tile this token sees
-                    if (seen <= 0) continue;
+                    for (int token = row0 / p.Hg; token <= j1; ++token) {
+                        const int seen = all_see + token - pos[j];              // keys of the tile this token sees
+                        if (seen <= 0) continue;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) own[x] = (row0 + 2 * t + x) / p.Hg == j;
-                    const uint32_t k0 = (2 * t < seen ? 0xFFFFu : 0u) | (2 * t + 1 < seen ? 0xFFFF0000u : 0u);
-                    const uint32_t k1 = (2 * t + 8 < seen ? 0xFFFFu : 0u) | (2 * t + 9 < seen ? 0xFFFF0000u : 0u);
-                    value_product<FP8, RW, true>(v_slot, lane, ph, pl, o, k0, k1, own);
+                        for (int x = 0; x < 2; ++x) own[x] = (row0 + 2 * t + x) / p.Hg == token;
+                        const uint32_t k0 = (2 * t < seen ? 0xFFFFu : 0u) | (2 * t + 1 < seen ? 0xFFFF0000u : 0u);
+                        const uint32_t k1 = (2 * t + 8 < seen ? 0xFFFFu : 0u) | (2 * t + 9 < seen ? 0xFFFF0000u : 0u);
+                        value_product<FP8, RW, true>(v_slot, lane, ph, pl, o, k0, k1, own);
+                    }
                 }
             }
             __syncwarp();
