@@ -160,9 +160,9 @@ __global__ void __launch_bounds__(kSelectThreads, 4) page_select_kernel(const __
             x.scale[i] = 0.0f;
             if (x.page[i] >= 0) {
                 const int64_t at = (int64_t)x.page[i] * p.Hkv + h;
-                x.lo[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + t);
-                x.hi[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + at * kD) + 4 + t);
-                x.scale[i] = __ldg(p.code_scales + at);
+                x.lo[i] = *(reinterpret_cast<const uint4*>(p.codes + at * kD) + t);
+                x.hi[i] = *(reinterpret_cast<const uint4*>(p.codes + at * kD) + 4 + t);
+                x.scale[i] = p.code_scales[at];
             }
         }
     };

@@ -118,7 +118,7 @@ def paged_decode_attention(query, k_pages, v_pages, block_table, seq_lens, scali
     With ``pages`` (int32 [B, Hkv, width]) and ``page_counts`` (int32 [B, Hkv]), both contiguous, a KV head attends
     only the first ``page_counts`` logical pages of its list, in any order; a page listed twice counts twice.
 
-    Returns the output in the shape of ``query`` (``out``, which may be a strided view, if given), and with
+    Returns the output in the shape of ``query`` (``out``, which may be a strided view or ``query`` itself, if given), and with
     ``return_lse`` also the natural logarithm of the softmax sums, fp32 of shape ``query.shape[:-1]``.  A row that
     sees nothing is 0, its logarithm -inf.  Scores, softmax and sums are 32-bit; results depend on the lengths
     in the batch only through the order of sums."""

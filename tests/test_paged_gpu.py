@@ -646,3 +646,51 @@ def test_first_call_inside_a_capture_is_refused():
         paged._status.update(kept)
     torch.cuda.synchronize()
     aa.paged_decode_attention(q, k, v, table, lens)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("page,n,H,Hkv", [(16, 1, 8, 2), (256, 1, 8, 2), (16, 6, 8, 2), (64, 16, 4, 2), (128, 9, 8, 2)])
+def test_picked_pages_of_all_sizes_and_rows(page, n, H, Hkv, fp8):
+    """Lists over pages smaller and larger than a step of the kernel, for one to many tiles of rows, long enough to be cut."""
+    g = torch.Generator().manual_seed(page + n)
+    lens = [40 * page - 3, 7 * page + 1, 150 * 16]
+    q, k, v, ks, vs, table, lens = _decode_case(page, lens, page, H, Hkv, n, fp8)
+    live = -(-lens // page)
+    width = int(live.max())
+    pages = torch.full((3, Hkv, width), -1, dtype=torch.int32)
+    counts = torch.zeros((3, Hkv), dtype=torch.int32)
+    for b in range(3):
+        for h in range(Hkv):
+            c = int(torch.randint(1, int(live[b]) + 1, (1,), generator=g))
+            pages[b, h, :c] = torch.randperm(int(live[b]), generator=g)[:c].int()
+            counts[b, h] = c
+    out, lse = _run(q, k, v, ks, vs, table, lens, pages=pages.cuda(), page_counts=counts.cuda())
+    assert_decode(out, lse, q, oracle.dequantised(k, ks), oracle.dequantised(v, vs), table, lens, fp8, pages=pages, page_counts=counts)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n,H,Hkv", [(16, 8, 1), (3, 20, 2), (11, 4, 4), (5, 16, 4)])
+def test_many_rows_over_long_sequences(n, H, Hkv, fp8):
+    """Several tiles of rows of sequences that are cut into parts."""
+    case = _decode_case(n, [5000, 777], 32, H, Hkv, n, fp8)
+    out, lse = _run(*case)
+    q, k, v, ks, vs, table, lens = case
+    assert_decode(out, lse, q, oracle.dequantised(k, ks), oracle.dequantised(v, vs), table, lens, fp8)
+
+
+def test_many_short_sequences():
+    """More sequences and heads than the kernel keeps at hand of a range, most of one unit."""
+    lens = [(i * 37) % 90 for i in range(700)]
+    case = _decode_case(5, lens, 16, 8, 4, 1, False)
+    out, lse = _run(*case)
+    q, k, v, ks, vs, table, lens = case
+    assert_decode(out, lse, q, k.double(), v.double(), table, lens, False)
+
+
+def test_attention_in_place_of_the_query():
+    """``out`` may be the query itself."""
+    case = _decode_case(6, [3000, 50, 700], 16, 8, 2, 2, False)
+    want, _ = _run(*case)
+    q, k, v, ks, vs, table, lens = _cuda(*case)
+    assert aa.paged_decode_attention(q, k, v, table, lens, out=q) is q
+    assert torch.equal(q, want)
