@@ -158,7 +158,8 @@ int make_page_map(CUtensorMap* map, const aa::paged::Pool& pool, const aa_paged_
 struct AttendPlan {
     int log2_page, rows, row_tiles, tiles8;       // tiles8: tiles of 8 rows one CTA holds (1 .. 4)
     int ctas, unit_keys;
-    bool split;                                   // whether an entry can be cut at all
+    bool whole;                                   // ranges of whole entries
+    bool split;                                   // an entry can be cut, and parts may have to be added up
     size_t o_off, ml_off, cut_off, bytes;
 };
 
@@ -202,9 +203,14 @@ int plan_attend(const aa_paged_attend_t* a, AttendPlan& pl) {
     const int64_t units = ceil_div(keys, pl.unit_keys);
     if (entries * units > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
     const int64_t most = (int64_t)dev.sms * aa::paged::kCtasPerSm;
-    pl.ctas = (int)(entries * units < most ? entries * units : most);
+    // Entries of few units stay whole: a CTA takes about 1 us a unit of 8 rows, the second kernel that would add up their parts
+    // 2.3 us.  One sequence of up to 120 tokens, 8 heads: 6.7 us whole, 8.9 us cut; 16 sequences of up to 250: 9.1 and 10.8; but
+    // one of 380 tokens (6 units): 10.9 and 8.8.
+    pl.whole = units <= (pl.tiles8 == 1 && 2 * entries >= dev.sms ? 4 : 2);
+    const int64_t pieces = pl.whole ? entries : entries * units;
+    pl.ctas = (int)(pieces < most ? pieces : most);
     if (pl.ctas > 512) pl.ctas = 512;             // the kernel's 32-bit ranges
-    pl.split = units > 1 && pl.ctas > 1;
+    pl.split = !pl.whole && pl.ctas > 1;
     const size_t parts = pl.split ? (size_t)pl.ctas * 2 * 8 * pl.tiles8 : 0;
     pl.o_off = 0;
     pl.ml_off = align256(parts * aa::kD * sizeof(float));
@@ -374,6 +380,7 @@ int aa_paged_attend(const aa_paged_attend_t* a, void* stream) {
     p.B = c.B; p.H = a->H; p.Hkv = c.Hkv; p.Hg = a->H / c.Hkv; p.nq = a->Nq;
     p.rows = pl.rows;
     p.row_tiles = pl.row_tiles;
+    p.whole = pl.whole;
     const double scale = a->sm_scale != 0.0 ? a->sm_scale : 1.0 / sqrt((double)c.D);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);

@@ -83,6 +83,7 @@ struct AttendParams {
     int B, H, Hkv, Hg, nq;
     int rows, row_tiles;                            // rows = nq * Hg, in tiles of 8 * RW
     float scale_log2;                               // softmax scale times log2 e
+    bool whole;                                     // ranges end where entries do: nothing is cut
     float* part_o;                                  // [ctas, 2, 8 RW, 128]
     float2* part_ml;                                // [ctas, 2, 8 RW]
     int2* cuts;                                     // [ctas]: (entry, parts) where a CTA's range is the first to start
@@ -319,7 +320,11 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     const int chunk = (entries + S::kThreads - 1) / S::kThreads;
     const int my_first = tid * chunk, my_end = min(entries, my_first + chunk);
     int mine = 0;
-    for (int e = my_first; e < my_end; ++e) mine += entry_units(p, e, S::kUnitKeys);
+    if (p.whole) {                                  // the line of entries is cut instead
+        mine = max(0, my_end - my_first);
+    } else {
+        for (int e = my_first; e < my_end; ++e) mine += entry_units(p, e, S::kUnitKeys);
+    }
     int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     }
     const int ctas = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= ctas) {
-        if (tid == 0) p.cuts[blockIdx.x] = make_int2(-1, 0);
+        if (tid == 0 && !p.whole) p.cuts[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     // CTA c owns the units [total c / ctas, total (c + 1) / ctas), in 32-bit arithmetic (ctas is at most 512)
@@ -345,9 +350,14 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     const int begin = range_start(blockIdx.x), end = range_start(blockIdx.x + 1);
     if (begin >= before && begin < before + mine) {
         int e = my_first, at = before;
-        for (int n = entry_units(p, e, S::kUnitKeys); at + n <= begin; n = entry_units(p, e, S::kUnitKeys)) {
-            at += n;
-            ++e;
+        if (p.whole) {
+            e += begin - before;
+            at = begin;
+        } else {
+            for (int n = entry_units(p, e, S::kUnitKeys); at + n <= begin; n = entry_units(p, e, S::kUnitKeys)) {
+                at += n;
+                ++e;
+            }
         }
         s_sum[S::kWarps + 1] = e;
         s_sum[S::kWarps + 2] = begin - at;
@@ -357,9 +367,9 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     if (before < end && before + mine > begin) {
         int at = before;
         for (int e = my_first; e < my_end && at < end && e - first_entry < kSegments; ++e) {
-            const int n = chunk == 1 ? mine : entry_units(p, e, S::kUnitKeys);
+            const int n = chunk == 1 && !p.whole ? mine : entry_units(p, e, S::kUnitKeys);
             if (e >= first_entry) segments[e - first_entry] = make_int2(n, seq_len(p.c, e / p.row_tiles / p.Hkv));
-            at += n;
+            at += p.whole ? 1 : n;
         }
     }
     if (blockIdx.x == 0)                            // the row of the block table bounds a sequence: report a longer one
@@ -368,10 +378,14 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
     __syncthreads();
 
     int left = end - begin;                         // units to do, at least one
+    if (p.whole) {
+        left = 0;
+        for (int e = begin; e < end; ++e) left += e - begin < kSegments ? segments[e - begin].x : entry_units(p, e, S::kUnitKeys);
+    }
     Cursor now;
     enter(p, now, first_entry, S::kUnitKeys, segments, first_entry);
     now.unit = first_unit;
-    if (tid == 0) {
+    if (tid == 0 && !p.whole) {
         const int starts = begin - first_unit;
         int2 cut = make_int2(-1, 0);
         if (first_unit > 0 && range_start(blockIdx.x - 1) <= starts) {
