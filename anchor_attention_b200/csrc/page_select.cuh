@@ -8,14 +8,15 @@
 // page, and come out in ascending order.
 //
 // A cluster of blocks works on one (sequence, KV head).  Its warps score 16 pages at a time, four lanes a page, with
-// four-byte dot products (the 8-bit matrix instruction took 34 SM cycles for 16 pages and 32 bytes), and leave the scores as
-// ordered 32-bit keys in the first block's shared memory; that block finds the last key that gets in by counting over
-// 11 + 11 + 10 bits and writes the list.  The scores are a few dependent loads per page, so a small batch is a matter of
-// latency: eight blocks share a sequence there, and each warp has 32 pages' loads in flight.
+// four-byte dot products (with the loads and the counting left out, the 8-bit matrix instructions took 3.7 of the batch's
+// 13.3 us), and leave the scores as ordered 32-bit keys in the first block's shared memory; that block finds the last key
+// that gets in by counting over 11 + 11 + 10 bits and writes the list.  The scores are a few dependent loads per page, so a
+// small batch is a matter of latency: eight blocks share a sequence there, and each warp has 32 pages' loads in flight.
 //
 // Measured (B200, whole calls): one sequence of 131072 tokens in pages of 64 8.7 us; 32 of up to 65536 in pages of 32 25 us for
-// 44 MB, where a kernel that only reads the same rows takes 11 to 12: the longest sequence's cluster is the last, and lengths, page
-// numbers, codes and counts wait for one another.  One block a sequence 28 to 30 us, four 28, eight 33.
+// 45 MB; a kernel that only reads 42 MB in rows of 128 bytes at random takes 10 to 13.  The rest is unequal lengths and a chain
+// of waits: lengths, page numbers, codes, counts.  Blocks for a sequence and head of that batch, on the GPU: one 28.0 us,
+// two 24.4 (what the rule takes), four 27.7, eight 32.8.
 #pragma once
 #include "paged_common.cuh"
 

@@ -14,8 +14,8 @@
 // d + 64 of a rotation.  For prompts a block takes several heads of a page, so that a row's cosines and sines are read once
 // for all of them and two heads' loads are in flight while the page number arrives; a single token's append is
 // latency alone and takes a block for every head.  Measured (B200): 26667 tokens of five prompts, 32/8 heads, bf16 124 us,
-// 5.8 TB/s of reads and writes mixed, 4 us of them for the means; 14232 tokens into e4m3 pages, 28/4 heads, 55 us, 4.6 TB/s (one head's loads
-// in flight instead of two: 55 against 57 us; two heads for bf16: 124 against 128 us); 64 single tokens 3 us on the GPU.
+// 5.8 TB/s of reads and writes mixed, 4 us of them for the means; 14232 tokens into e4m3 pages, 28/4 heads,
+// 55 us, 4.6 TB/s (one head's loads in flight instead of two: 55 against 57 us; two for bf16: 124 against 128 us); 64 single tokens 3 us on the GPU.
 #pragma once
 #include <cuda_fp8.h>
 

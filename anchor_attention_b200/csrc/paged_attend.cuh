@@ -21,11 +21,14 @@
 // Scores are computed transposed, S^T = K Q^T: the keys fill the 16 rows of the matrix instruction and 8 queries its
 // columns, so a group of 4 wastes half of a tile of 8 instead of three quarters of one of 16; the
 // probabilities then need one 8x8 transpose to become the operand of O^T = V^T P^T.  mma.sync is enough: a
-// tensor-core tile of 128 rows would be filled with padding, and the tensor pipe is busy a seventh of the time.
+// tensor-core tile of 128 rows would be filled with padding, and the tensor pipe is busy 16 (bf16) to 38 % of the time
+// (three row tiles).
 //
 // Measured (B200, whole calls): 32 sequences of up to 32768 tokens, 32/8 heads: bf16 357 us, 6.8 TB/s; e4m3 188 us, 6.4 TB/s;
-// one sequence of 131072 tokens 87.5 us, 6.1 TB/s; 16 of up to 4001 tokens 23 us, of which 10 stream and the rest starts and ends
-// the call; five new tokens for 8 sequences of up to 16001 75 us, bound by latencies inside a tile.
+// one sequence of 131072 tokens 87.5 us, 6.1 TB/s; 16 of up to 4001 tokens 23 us, where the bytes alone
+// take 10; five new tokens for 8 sequences of up to 16001 75 us, bound by latencies inside a tile.
+// Without the join kernel (its results then incomplete) calls take 2 us less on the GPU for one short sequence, 3 to 5 us
+// for most, 8 us for the five new tokens.
 //
 // Accuracy.  Scores, softmax state and outputs are held in 32 bits.  With bf16 pages a probability goes into
 // the second product as the sum of two bf16 values (15 bits), so that only the output is rounded to 8;

@@ -68,7 +68,7 @@ def _new_status_word(index: int) -> torch.Tensor:
 def check_paged_status(device=None) -> None:
     """Synchronises the current stream and raises if a call since the last check met a page number outside the
     pool, a list entry outside its sequence, or a sequence longer than its row of the block table (or than
-    the rotary tables)."""
+    the rotary tables), or if a bounded wait of the attention kernel gave up."""
     index = torch.device(device).index if device is not None else None
     index = torch.cuda.current_device() if index is None else index
     word = _status.get(index)
