@@ -54,6 +54,11 @@ const at::Tensor& optional_tensor(PyObject* o, const char* name) {
     static const at::Tensor none;
     return o == Py_None ? none : tensor(o, name);
 }
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v == 1;
+}
 int64_t integer(PyObject* o) {
     const int64_t v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) throw python_error();
@@ -231,7 +236,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                          &query = optional_tensor(args[7], "query"), &cos = optional_tensor(args[8], "cos"),
                          &sin = optional_tensor(args[9], "sin"), &codes = optional_tensor(args[12], "key_codes"),
                          &scales = optional_tensor(args[13], "key_code_scales");
-        const bool return_key = PyObject_IsTrue(args[14]) == 1;
+        const bool return_key = truth(args[14]);
         const at::Device device = k.device();
         aa_paged_append_t a{};
         a.cache = make_cache(k, v, tensor(args[4], "block_table"), tensor(args[5], "seq_lens"),
@@ -306,7 +311,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor &query = tensor(args[0], "query"), &k = tensor(args[1], "k_pages"), &v = tensor(args[2], "v_pages"),
                          &pages = optional_tensor(args[8], "pages"), &counts = optional_tensor(args[9], "page_counts"),
                          &out_in = optional_tensor(args[10], "out");
-        const bool return_lse = PyObject_IsTrue(args[11]) == 1;
+        const bool return_lse = truth(args[11]);
         const at::Device device = k.device();
         aa_paged_attend_t a{};
         a.cache = make_cache(k, v, tensor(args[3], "block_table"), tensor(args[4], "seq_lens"),

@@ -245,3 +245,17 @@ def test_oracle_selection_keeps_ends_and_breaks_ties_low():
     assert counts.item() == 5 and lists[0, 0].tolist() == [0, 2, 3, 8, 9]
     lists, counts = oracle.select(q.bfloat16(), codes, torch.ones(10, 1), table, [33], 5, 16)
     assert counts.item() == 3 and lists[0, 0].tolist() == [0, 1, 2, -1, -1]
+
+
+class _NoTruth:
+    def __bool__(self):
+        raise ValueError("no truth value")
+
+
+def test_flags_without_a_truth_value(lib):
+    t = _tensors()
+    with pytest.raises(ValueError, match="no truth value"):
+        aa.paged_kv_append(**t, return_key=_NoTruth())
+    attend = {n: t[n] for n in ("query", "k_pages", "v_pages", "block_table", "seq_lens")}
+    with pytest.raises(ValueError, match="no truth value"):
+        aa.paged_decode_attention(**attend, return_lse=_NoTruth())
