@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
     if (page_index < 0) return;
     const int rows = 1 << p.c.log2_page;
     const int first = page_index << p.c.log2_page;
-    const int lo = max(span.start, first), hi = min(span.end, first + rows);    // positions of this task
+    const int lo = max(span.start, first), hi = first + min(span.end - first, rows);    // positions of this task
     const int token0 = span.token - span.start;                                // token of position x: token0 + x
 
     // slots of 8 threads, a row each; where there are fewer rows, several heads go side by side
@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
 
     if ((int)blockIdx.y >= p.kv_blocks) {
         const int h0 = ((int)blockIdx.y - p.kv_blocks) * p.q_heads, h1 = min(h0 + p.q_heads, p.H);
-        for (int pos = lo + slot_row; pos < hi; pos += slot_rows) {
+        for (int i = slot_row; i < hi - lo; i += slot_rows) {
+            const int pos = lo + i;                    // lo + i + slot_rows could pass 2^31
             if (p.cos && pos >= p.rope_rows) {
                 beyond = true;
                 continue;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
     const bool in_table = page_index < p.c.table_width;
     const int page = in_table ? pool_page(p.c, b, page_index) : -1;
     // the page fills up: its mean is wanted, from shared memory where it fits
-    const bool fills = p.codes && page >= 0 && hi == first + rows && (!p.cos || hi <= p.rope_rows);
+    const bool fills = p.codes && page >= 0 && hi - first == rows && (!p.cos || hi <= p.rope_rows);
     const bool staged = fills && p.staged;
     constexpr int kRowBytes8 = FP8 ? 128 : 256;
     if (staged)                                     // rows of earlier calls
@@ -293,7 +294,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == kAppendThreads ? 3 : 4) pa
             reinterpret_cast<uint4*>(paged_append_smem + (h * rows + row) * kRowBytes8)[piece] =
                 reinterpret_cast<const uint4*>(p.c.k.ptr + page * p.c.k.page + (h0 + h) * p.c.k.head + row * p.c.k.row)[piece];
         }
-    for (int pos = lo + slot_row; pos < hi; pos += slot_rows) {
+    for (int i = slot_row; i < hi - lo; i += slot_rows) {
+        const int pos = lo + i;
         if (p.cos && pos >= p.rope_rows) {
             beyond = true;
             continue;

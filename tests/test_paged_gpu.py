@@ -694,3 +694,17 @@ def test_attention_in_place_of_the_query():
     q, k, v, ks, vs, table, lens = _cuda(*case)
     assert aa.paged_decode_attention(q, k, v, table, lens, out=q) is q
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_append_at_the_largest_length(ragged):
+    """Positions up to 2^31 - 2, whose page ends at 2^31: the keys lie beyond the table and are left out, the queries (not
+    rotated, so no position is beyond the tables) are copied."""
+    n = 1 if not ragged else 3
+    c = _append_case(8, [n], [0], 16, 4, 2, False, ragged=ragged)
+    c["lens"][0] = 2 ** 31 - 1
+    r = _append(c, rotate=False)
+    assert torch.equal(r["q"].cpu(), c["query"]) and torch.equal(r["k"].cpu(), c["k"]) and torch.equal(r["v"].cpu(), c["v"])
+    assert (r["codes"] == 55).all()
+    with pytest.raises(RuntimeError, match="longer"):
+        aa.check_paged_status()
