@@ -24,9 +24,10 @@
 // tensor-core tile of 128 rows would be filled with padding, and the tensor pipe is busy 16 (bf16) to 38 % of the time
 // (three row tiles).
 //
-// Measured (B200, whole calls): 32 sequences of up to 32768 tokens, 32/8 heads: bf16 357 us, 6.8 TB/s; e4m3 188 us, 6.4 TB/s;
+// Measured (B200, whole calls): 32 sequences of up to 32768 tokens, 32/8 heads: bf16 357 to 365 us, 6.6 to 6.8 TB/s; e4m3 188 to
+// 199 us, 6.1 to 6.4 TB/s;
 // one sequence of 131072 tokens 87.5 us, 6.1 TB/s; 16 of up to 4001 tokens 23 us, where the bytes alone
-// take 10; five new tokens for 8 sequences of up to 16001 75 us, bound by latencies inside a tile.
+// take 10; five new tokens for 8 sequences of up to 16001 74 to 79 us, bound by latencies inside a tile.
 // Without the join kernel (its results then incomplete) calls take 2 us less on the GPU for one short sequence, 3 to 5 us
 // for most, 8 us for the five new tokens.
 //
