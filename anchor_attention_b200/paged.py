@@ -61,8 +61,8 @@ def _new_status_word(index: int) -> torch.Tensor:
     device = torch.device("cuda", index)
     word = torch.zeros(1, dtype=torch.int32, device=device)
     torch.cuda.current_stream(device).synchronize()          # whatever stream comes next sees the zero
-    _status[index] = word
-    return word
+    # Another thread's first call may have got here during the wait: its word is kept, and both calls use it.
+    return _status.setdefault(index, word)
 
 
 def check_paged_status(device=None) -> None:
