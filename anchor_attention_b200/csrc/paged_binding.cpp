@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <limits>
 #include <optional>
 #include <string>
 
@@ -320,6 +321,8 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (args[5] != Py_None) {
             a.sm_scale = PyFloat_AsDouble(args[5]);
             if (PyErr_Occurred()) throw python_error();
+            // 0 stands for the default in the argument block; the smallest double is a scale of 0 in 32 bits
+            if (a.sm_scale == 0.0) a.sm_scale = std::numeric_limits<double>::denorm_min();
         }
         need_rows(query, "query", device);
         Queries q = make_queries(query, c.Hkv, c.B);

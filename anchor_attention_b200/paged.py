@@ -113,7 +113,8 @@ def paged_decode_attention(query, k_pages, v_pages, block_table, seq_lens, scali
                            return_lse: bool = False):
     """Attention of the last tokens of every sequence over a paged cache that holds them already.  ``query``
     [B, H, 128] (one new token) or [B, n, H, 128] with n up to 16 (row j is position ``seq_lens[b] - n + j`` and sees
-    positions up to its own); query head h reads KV head h // (H / Hkv); ``scaling`` defaults to 128 ** -0.5.
+    positions up to its own); query head h reads KV head h // (H / Hkv); ``scaling`` defaults to 128 ** -0.5 (0 gives
+    all keys the same weight).
 
     With ``pages`` (int32 [B, Hkv, width]) and ``page_counts`` (int32 [B, Hkv]), both contiguous, a KV head attends
     only the first ``page_counts`` logical pages of its list, in any order; a page listed twice counts twice.

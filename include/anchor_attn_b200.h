@@ -442,7 +442,7 @@ typedef struct aa_paged_attend {
     const int32_t *pages, *page_counts;
     void *workspace;
     size_t workspace_bytes;
-    double sm_scale;                   /* 0 => D^-0.5 */
+    double sm_scale;                   /* 0 => D^-0.5; any other number below 2^-151 is a scale of 0 (equal weights) */
     int32_t list_width, Nq, H;
     int32_t reserved;
 } aa_paged_attend_t;

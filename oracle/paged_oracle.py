@@ -32,7 +32,7 @@ def attend(query, k, v, block_table, seq_lens, scaling=None, pages=None, page_co
     B, n, H, _ = query.shape
     Hkv, page = k.shape[1], k.shape[2]
     group = H // Hkv
-    scaling = scaling or 128 ** -0.5
+    scaling = 128 ** -0.5 if scaling is None else scaling
     out = torch.zeros(query.shape, dtype=torch.float64)
     weight = torch.zeros(query.shape, dtype=torch.float64)
     lse = torch.full(query.shape[:3], -math.inf, dtype=torch.float64)
