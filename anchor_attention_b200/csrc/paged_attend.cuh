@@ -9,7 +9,7 @@
 // Work split.  An entry is one (sequence, KV head, tile of up to 32 rows); its keys are cut into units.  All
 // units of all entries form one line that is cut into as many equal ranges as there are CTAs, whatever the
 // lengths: a batch of unequal sequences and a single long one fill the GPU alike.  Where a cut falls inside an
-// entry, the CTAs on its sides leave (maximum, sum, unnormalised row) and paged_join_kernel adds them
+// entry, the CTAs on its sides leave (reference, sum, unnormalised row) and paged_join_kernel adds them
 // up in the order of the keys; results depend on the lengths alone, not on timing.  Entries of a few units stay whole.
 //
 // Inside a CTA a producer warp walks the units: it looks up their pages and has the TMA copy them (128-byte swizzle)
@@ -34,7 +34,9 @@
 // Accuracy.  Scores, softmax state and outputs are held in 32 bits.  With bf16 pages a probability goes into
 // the second product as the sum of two bf16 values (15 bits), so that only the output is rounded to 8;
 // the extra instructions hide behind the loads.  With e4m3 pages both products run in f16, in which every
-// code is exact and a probability keeps 11 bits; queries are scaled by a power of two per row to fit f16.
+// code is exact; queries are scaled by a power of two per row to fit f16.  A lane's probabilities are held relative to 2^15 at
+// its largest, so that f16 keeps 11 bits of those down to 2^-29 of it and loses none above 2^-40; the sum of the
+// denominator is of the values before that rounding.
 #pragma once
 #include "paged_common.cuh"
 #include "tc_ptx.cuh"
@@ -279,7 +281,7 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* to, int lane, const flo
     reinterpret_cast<uint2*>(to)[lane] = make_uint2(pack_bf16x2(none ? 0.0f : acc.x * f, none ? 0.0f : acc.y * f),
                                                     pack_bf16x2(none ? 0.0f : acc.z * f, none ? 0.0f : acc.w * f));
 }
-// The natural logarithm of a softmax sum from its maximum (log2 units) and the sum behind it.
+// The natural logarithm of a softmax sum from its reference (log2 units) and the sum behind it.
 __device__ __forceinline__ float log_sum(float top, float sum) {
     return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
@@ -296,6 +298,8 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                         const __grid_constant__ AttendParams p) {
     using S = Shape<FP8, RW>;
     constexpr int kStages = S::kStages, kDepth = S::kDepth;
+    // A state (m, l, o) stands for 2^m l and 2^m o; m is the running maximum less this, so a probability is at most 2^15 in f16.
+    constexpr float kLift = FP8 ? 15.0f : 0.0f;
     extern __shared__ __align__(1024) uint8_t paged_attend_smem[];
     float* comb = reinterpret_cast<float*>(paged_attend_smem + kRingBytes);
     // the last 512 bytes: barriers, lengths of this range's entries, tile positions of the stages, scratch of the start
@@ -554,7 +558,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                const float m_new = fmaxf(m[x], top);
+                const float m_new = fmaxf(m[x], top - kLift);
                 const float ref = m_new == -INFINITY ? 0.0f : m_new;       // a row that has seen nothing yet
                 corr[x] = fast_exp2(m[x] - ref);
                 m[x] = m_new;

@@ -52,3 +52,55 @@ def test_a_scale_of_zero_weighs_all_keys_alike(scaling, fp8):
         assert ((lse[b] - math.log(n)).abs() <= 2.0 ** -20 + 2.0 ** -22 * math.log(n)).all()
     ref = oracle.attend(q, oracle.dequantised(k, ks), values, table, lens_t, scaling=scaling)
     assert (ref[1][0] - math.log(400)).abs().max() < 1e-12
+
+
+def _own_key_bounds(query, out, lse, weight, spread, lens, v):
+    """decode_bounds of an e4m3 cache with the part that does not scale with a row's values taken from the sequence's own
+    keys: a weight is held in f16 relative to 2^15 at its lane's largest, so what rounds to nothing is below 2^-40 of it.
+    A score is off by 128 * 2^-23 of its sum of sizes (128 exact products added in 32 bits), a query's f16 copy by 2^-33 of its
+    row's largest value an element; scale, exponential and its argument add 2^-15; a weight in f16 2^-11; the output 2^-8."""
+    d = 128 * 2.0 ** -23 * spread + 2.0 ** -15 + 128 * 2.0 ** -33 * spread
+    nothing = 2.0 ** -40 * lens.double() * v.abs().max()
+    tol_out = 2.0 ** -8 * out.abs() + (2 * d + 2.0 ** -11)[..., None] * weight + nothing[:, None, None, None] + 1e-30
+    return tol_out, d + 2.0 ** -20 + 2.0 ** -22 * torch.where(lse.isfinite(), lse.abs(), torch.zeros_like(lse))
+
+
+def test_e4m3_tail_behind_strong_keys():
+    """A few strong keys at the front and thousands of others at 2^-17 to 2^-25 of their weight, one level for each KV head;
+    some values come from the others alone, so what is lost of their weights shows at full size.  37 sequences of 8 heads
+    (all on the same pages) leave every entry whole, so that the strong keys' lanes see most of the others."""
+    Hkv, page, n = 8, 64, 16384
+    g = torch.Generator().manual_seed(4)
+    k = torch.zeros(n // page, Hkv, page, 128)
+    k[..., 0] = -2.0 - torch.arange(Hkv).float()[None, :, None]
+    k[:2, :, ::16, 0] = 16.0                                # every 16th of the first 128 positions
+    v = (torch.randint(4, 13, k.shape, generator=g) / 8).float()
+    v[..., :64] = 0.0
+    v[:2, :, ::16] = 0.0
+    v[:2, :, ::16, :64] = 1.0
+    k, v = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+    ones = torch.ones(Hkv)
+    q = torch.zeros(37, 1, Hkv, 128)
+    q[..., 0] = 1.0
+    q = q.bfloat16()
+    table = torch.arange(n // page, dtype=torch.int32)[None].repeat(37, 1)
+    lens = torch.full((37,), n, dtype=torch.int32)
+    scaling = 0.97 * math.log(2)
+    got, got_lse = _run(q, k, v, ones, ones, table, lens, scaling=scaling)
+    out, lse, weight, spread = oracle.attend(q[:1], k.double(), v.double(), table[:1], lens[:1], scaling=scaling)
+    tol_out, tol_lse = _own_key_bounds(q[:1], out, lse, weight, spread, lens[:1], v.double())
+    assert bool((out[..., 64:] > 2.0 ** -16).all())
+    for b in range(37):
+        assert ((got[b].double().cpu() - out[0]).abs() <= tol_out[0]).all()
+        assert ((got_lse[b].double().cpu() - lse[0]).abs() <= tol_lse[0]).all()
+
+
+@pytest.mark.parametrize("lens,H,Hkv", [([20000], 8, 1), ([9001, 1, 12000], 8, 2), ([4097] * 40, 4, 4)])
+def test_e4m3_within_the_bounds_of_the_sequences_own_keys(lens, H, Hkv):
+    q, k, v, ks, vs, table, lens = _case(3, lens, 64, H, Hkv, 1, True)
+    got, got_lse = _run(q, k, v, ks, vs, table, lens)
+    values = oracle.dequantised(v, vs)
+    out, lse, weight, spread = oracle.attend(q, oracle.dequantised(k, ks), values, table, lens)
+    tol_out, tol_lse = _own_key_bounds(q, out, lse, weight, spread, lens, values)
+    assert ((got.double().cpu() - out).abs() <= tol_out).all()
+    assert ((got_lse.double().cpu() - lse).abs() <= tol_lse).all()
