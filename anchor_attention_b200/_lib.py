@@ -22,7 +22,7 @@ EXPORTS = [
     "aa_block_sparse_check_status", "aa_validate_lists", "aa_step2_stripes_static_check_status",
     "aa_peer_barrier", "aa_dense_causal_attend", "aa_rope_dispatch",
     "aa_paged_append", "aa_paged_attend", "aa_paged_attend_workspace_bytes", "aa_page_select",
-    "aa_paged_check_status",
+    "aa_paged_check_status", "aa_selftest_paged_wait",
 ]
 MAX_PEERS = 8
 STATIC_SCRATCH_BYTES = 8 << 20
@@ -186,7 +186,7 @@ def load():
         getattr(lib, name).argtypes = [PB, ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
     for name, struct in (("aa_paged_append", AAPagedAppend), ("aa_paged_attend", AAPagedAttend),
-                         ("aa_page_select", AAPageSelect)):
+                         ("aa_page_select", AAPageSelect), ("aa_selftest_paged_wait", AAPagedAttend)):
         getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
     lib.aa_paged_attend_workspace_bytes.argtypes = [ctypes.POINTER(AAPagedAttend), ctypes.POINTER(ctypes.c_size_t)]

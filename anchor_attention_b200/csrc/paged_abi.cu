@@ -243,6 +243,52 @@ int launch_attend_rows(const CUtensorMap& km, const CUtensorMap& vm, const aa::p
     }
 }
 
+// wait_polls: after which a computing warp gives up on a copy
+int run_attend(const aa_paged_attend_t* a, uint32_t wait_polls, void* stream) {
+    AttendPlan pl;
+    int rc = plan_attend(a, pl);
+    if (rc) return rc;
+    const aa_paged_cache_t& c = a->cache;
+    rc = check_pools(c);
+    if (rc) return rc;
+    if (!a->q || !a->out) return AA_ERR_NULL;
+    for (int64_t s : {a->q_stride_b, a->q_stride_n, a->q_stride_h, a->o_stride_b, a->o_stride_n, a->o_stride_h})
+        if (bad_stride(s)) return AA_ERR_STRIDE;
+    if (misaligned(a->q) || misaligned(a->out)) return AA_ERR_STRIDE;
+    if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < pl.bytes) return AA_ERR_WORKSPACE;
+
+    aa::paged::AttendParams p;
+    p.c = view(c, pl.log2_page);
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.q_sb = a->q_stride_b; p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h;
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.o_sb = a->o_stride_b; p.o_sn = a->o_stride_n; p.o_sh = a->o_stride_h;
+    p.lse = a->lse;
+    p.pages = a->pages;
+    p.page_counts = a->page_counts;
+    p.list_width = a->list_width;
+    p.B = c.B; p.H = a->H; p.Hkv = c.Hkv; p.Hg = a->H / c.Hkv; p.nq = a->Nq;
+    p.rows = pl.rows;
+    p.row_tiles = pl.row_tiles;
+    p.whole = pl.whole;
+    const double scale = a->sm_scale != 0.0 ? a->sm_scale : 1.0 / sqrt((double)c.D);
+    p.scale_log2 = (float)(scale * 1.4426950408889634);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
+    p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
+    p.cuts = reinterpret_cast<int2*>(ws + pl.cut_off);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int box = c.page_size < pl.unit_keys ? c.page_size : pl.unit_keys;
+    p.log2_box = 31 - __builtin_clz((unsigned)box);
+    p.wait_polls = wait_polls;
+    CUtensorMap k_map, v_map;
+    rc = make_page_map(&k_map, p.c.k, c, box, &p.k_order);
+    if (!rc) rc = make_page_map(&v_map, p.c.v, c, box, &p.v_order);
+    if (rc) return rc;
+    return c.cache_dtype == AA_E4M3 ? launch_attend_rows<true>(k_map, v_map, p, pl, st)
+                                    : launch_attend_rows<false>(k_map, v_map, p, pl, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -354,49 +400,9 @@ int aa_paged_attend_workspace_bytes(const aa_paged_attend_t* a, size_t* bytes) {
     return AA_OK;
 }
 
-int aa_paged_attend(const aa_paged_attend_t* a, void* stream) {
-    AttendPlan pl;
-    int rc = plan_attend(a, pl);
-    if (rc) return rc;
-    const aa_paged_cache_t& c = a->cache;
-    rc = check_pools(c);
-    if (rc) return rc;
-    if (!a->q || !a->out) return AA_ERR_NULL;
-    for (int64_t s : {a->q_stride_b, a->q_stride_n, a->q_stride_h, a->o_stride_b, a->o_stride_n, a->o_stride_h})
-        if (bad_stride(s)) return AA_ERR_STRIDE;
-    if (misaligned(a->q) || misaligned(a->out)) return AA_ERR_STRIDE;
-    if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < pl.bytes) return AA_ERR_WORKSPACE;
+int aa_paged_attend(const aa_paged_attend_t* a, void* stream) { return run_attend(a, aa::tc::kSpinLimit, stream); }
 
-    aa::paged::AttendParams p;
-    p.c = view(c, pl.log2_page);
-    p.q = static_cast<const __nv_bfloat16*>(a->q);
-    p.q_sb = a->q_stride_b; p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h;
-    p.out = static_cast<__nv_bfloat16*>(a->out);
-    p.o_sb = a->o_stride_b; p.o_sn = a->o_stride_n; p.o_sh = a->o_stride_h;
-    p.lse = a->lse;
-    p.pages = a->pages;
-    p.page_counts = a->page_counts;
-    p.list_width = a->list_width;
-    p.B = c.B; p.H = a->H; p.Hkv = c.Hkv; p.Hg = a->H / c.Hkv; p.nq = a->Nq;
-    p.rows = pl.rows;
-    p.row_tiles = pl.row_tiles;
-    p.whole = pl.whole;
-    const double scale = a->sm_scale != 0.0 ? a->sm_scale : 1.0 / sqrt((double)c.D);
-    p.scale_log2 = (float)(scale * 1.4426950408889634);
-    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-    p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
-    p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
-    p.cuts = reinterpret_cast<int2*>(ws + pl.cut_off);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int box = c.page_size < pl.unit_keys ? c.page_size : pl.unit_keys;
-    p.log2_box = 31 - __builtin_clz((unsigned)box);
-    CUtensorMap k_map, v_map;
-    rc = make_page_map(&k_map, p.c.k, c, box, &p.k_order);
-    if (!rc) rc = make_page_map(&v_map, p.c.v, c, box, &p.v_order);
-    if (rc) return rc;
-    return c.cache_dtype == AA_E4M3 ? launch_attend_rows<true>(k_map, v_map, p, pl, st)
-                                    : launch_attend_rows<false>(k_map, v_map, p, pl, st);
-}
+int aa_selftest_paged_wait(const aa_paged_attend_t* a, void* stream) { return run_attend(a, 0, stream); }
 
 int aa_page_select(const aa_page_select_t* a, void* stream) {
     if (!a) return AA_ERR_NULL;

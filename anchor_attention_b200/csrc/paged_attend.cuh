@@ -101,6 +101,7 @@ struct AttendParams {
                                                     // share; else (-1, 0)
     MapOrder k_order, v_order;
     int log2_box;                                   // keys of one copy: the smaller of page and unit
+    uint32_t wait_polls;                            // after which a computing warp gives up on a copy
 };
 
 // Keys an entry streams over (list entries count as whole pages) and the units they make; an empty one still
@@ -421,10 +422,12 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
         const uint32_t box_at = part * S::kPartBytes + box * box_bytes;
         int pos = 0, page = lane < S::kTiles ? locate(p, now, S::kTiles, lane, pos) : -1;
         uint32_t stage = 0, parity = 1;             // of the stage's previous use: the first pass waits for nothing
+        int issued = 0;
         for (int i = 0; i < left; ++i) {
-            tc::mbar_wait(empty(stage), parity, abort_flag);
-            __syncwarp();
-            if (*abort_flag) break;
+            // One answer for the warp, whose lanes exchange pages below.  A computing warp that gives up raises the flag before
+            // it hands the stage back, so a stage whose copy may still be in flight is not filled again.
+            const bool may_fill = tc::mbar_wait(empty(stage), parity, abort_flag) && !*abort_flag;
+            if (!__all_sync(0xFFFFFFFFu, may_fill)) break;
             const int first_tile = (box << p.log2_box) / kTileKeys;
             const int box_page = __shfl_sync(0xFFFFFFFFu, page, first_tile & 31);
             const int box_pos = __shfl_sync(0xFFFFFFFFu, pos, first_tile & 31);
@@ -441,6 +444,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 for (int d = 0; d < 3; ++d) at[d] = order.row == d ? row : order.head == d ? now.h : box_page;
                 tc::tma_load_4d(ring + stage * S::kUnitBytes + box_at, map, full(stage), x, at[0], at[1], at[2]);
             }
+            issued = i + 1;
             if (i + 1 < left) {
                 if (++now.unit == now.units) {
                     enter(p, now, now.entry + 1, S::kUnitKeys, segments, first_entry);
@@ -453,11 +457,12 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 parity ^= 1;
             }
         }
-        if (*abort_flag) {
-            // a wait gave up: let the copies in flight land before shared memory is handed on
-            for (int i = 0; i < kStages; ++i) tc::mbar_wait(full(i), 0, abort_flag), tc::mbar_wait(full(i), 1, abort_flag);
-            if (lane == 0) raise_status(p.c, kStatusTimeout);
-        }
+        // The block's shared memory is not handed on before the last copies have landed: a computing warp that gives up on
+        // one of them does not wait for it.
+        bool all_landed = true;
+        for (int i = max(issued - kStages, 0); i < issued; ++i)
+            all_landed = tc::mbar_drain(full(i % kStages), (i / kStages) & 1) && all_landed;
+        if (issued < left || !all_landed) raise_status(p.c, kStatusTimeout);
         return;
     }
 
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
 
         for (int step = 0; step < todo; ++step) {
             const uint32_t free_bar = empty(stage);
-            const bool landed = tc::mbar_wait(full(stage), parity, abort_flag);
+            const bool landed = tc::mbar_wait(full(stage), parity, abort_flag, p.wait_polls);
             int pos[kDepth];
             bool any = false;
 #pragma unroll
@@ -508,6 +513,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 parity ^= 1;
             }
             if (!__all_sync(0xFFFFFFFFu, any)) {
+                __syncwarp();                       // a raised flag is visible before the stage is handed back
                 if (lane == 0) tc::mbar_arrive(free_bar);
                 continue;
             }
@@ -688,6 +694,9 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
             compute_sync();
         }
     }
+    // A wait of this block gave up, and some keys are missing above.  A warp whose own wait did sees its flag here, whether or not
+    // the producer is still there to report it.
+    if (*abort_flag) raise_status(p.c, kStatusTimeout);
 }
 
 // Adds up the parts of the entries that a cut of the line went through.  Block (c - 1, r) takes row r of the entry that CTA

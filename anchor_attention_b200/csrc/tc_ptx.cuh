@@ -39,8 +39,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // the CTA's abort flag and gives up; all other waiters see the flag and leave too.
 constexpr uint32_t kSpinLimit = 1u << 22;
 
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          uint32_t limit = kSpinLimit) {
+    for (uint32_t i = 0; i < limit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (i >= 128) {
             __nanosleep(64);
@@ -48,6 +49,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
     *abort_flag = 1;
+    return false;
+}
+// The wait for a copy that has been issued, before shared memory is given up: it goes on whatever the abort flag
+// says, up to the same limit.
+__device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (i >= 128) __nanosleep(64);
+    }
     return false;
 }
 

@@ -448,6 +448,9 @@ typedef struct aa_paged_attend {
 } aa_paged_attend_t;
 int aa_paged_attend_workspace_bytes(const aa_paged_attend_t *a, size_t *bytes);
 int aa_paged_attend(const aa_paged_attend_t *a, void *stream);
+/* Self-test of the bounded waits: the same call, but its computing warps give up on every copy at once.  Nothing faults and
+ * the launch ends as usual; out and lse are of no use, and aa_paged_check_status returns AA_ERR_DEVICE_TIMEOUT. */
+int aa_selftest_paged_wait(const aa_paged_attend_t *a, void *stream);
 
 /*
  * The pages of every sequence and KV head to attend: the first keep_first and the last keep_last pages, then those of

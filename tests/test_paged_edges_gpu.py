@@ -1,10 +1,12 @@
 """Edge cases of the paged cache on the GPU: arguments and cache contents at the borders of what the functions accept."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import anchor_attention_b200 as aa
+from anchor_attention_b200 import _lib
 from oracle import paged_oracle as oracle
 from paged_util import make_pool, make_table
 
@@ -104,3 +106,50 @@ def test_e4m3_within_the_bounds_of_the_sequences_own_keys(lens, H, Hkv):
     tol_out, tol_lse = _own_key_bounds(q, out, lse, weight, spread, lens, values)
     assert ((got.double().cpu() - out).abs() <= tol_out).all()
     assert ((got_lse.double().cpu() - lse).abs() <= tol_lse).all()
+
+
+# ------------------------------------------------------------------------------------------------ bounded waits
+def _attend_block(q, k, v, ks, vs, table, lens, out, lse, status):
+    a = _lib.AAPagedAttend()
+    c = a.cache
+    c.k_pages, c.v_pages, c.block_table, c.seq_lens, c.status = (t.data_ptr() for t in (k, v, table, lens, status))
+    for name, t in (("k", k), ("v", v)):
+        for axis, stride in zip(("page", "head", "row"), t.stride()):
+            setattr(c, f"{name}_stride_{axis}", stride)
+    if ks is not None:
+        c.k_scale, c.v_scale, c.cache_dtype = ks.data_ptr(), vs.data_ptr(), _lib.AA_E4M3
+    c.table_stride, c.table_width = table.stride(0), table.shape[1]
+    c.pages, c.Hkv, c.page_size, c.D, c.B = k.shape[0], k.shape[1], k.shape[2], 128, table.shape[0]
+    a.q, a.out, a.lse, a.Nq, a.H = q.data_ptr(), out.data_ptr(), lse.data_ptr(), q.shape[1], q.shape[2]
+    a.q_stride_b, a.q_stride_n, a.q_stride_h, _ = q.stride()
+    a.o_stride_b, a.o_stride_n, a.o_stride_h, _ = out.stride()
+    need = ctypes.c_size_t()
+    assert _lib.load().aa_paged_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(need)) == 0
+    workspace = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+    return a, workspace
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lens,H,Hkv,n", [
+    ([5], 8, 2, 1),                 # one unit: the producer has issued everything before anyone gives up
+    ([200, 90, 0], 8, 2, 1),        # fewer units than stages
+    ([30000], 8, 1, 1),             # more units than stages, cut into parts
+    ([9000] * 40, 8, 8, 1),         # many units a block
+    ([4000, 17], 8, 2, 5), ([4000, 17], 8, 1, 4),
+])
+def test_a_computing_warp_that_gives_up_is_reported(lens, H, Hkv, n, fp8):
+    """The self-test's computing warps give up on every copy: the call ends, its copies have landed before its blocks do, the status says
+    so, and the same call with ordinary limits is right afterwards."""
+    q, k, v, ks, vs, table, lens_t = [None if t is None else t.cuda() for t in _case(5, lens, 16, H, Hkv, n, fp8)]
+    want, want_lse = aa.paged_decode_attention(q, k, v, table, lens_t, k_scale=ks, v_scale=vs, return_lse=True)
+    out, lse = torch.empty_like(want), torch.empty_like(want_lse)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, workspace = _attend_block(q, k, v, ks, vs, table, lens_t, out, lse, status)
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for _ in range(3):
+        assert lib.aa_selftest_paged_wait(ctypes.byref(a), stream) == 0
+        assert lib.aa_paged_check_status(status.data_ptr(), stream) == -11
+        assert lib.aa_paged_attend(ctypes.byref(a), stream) == 0
+        assert lib.aa_paged_check_status(status.data_ptr(), stream) == 0
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
