@@ -59,9 +59,10 @@ __device__ __forceinline__ int pool_page(const Cache& c, int b, int logical) {
 }
 
 // ---- quotients
-// Division by one number for many: q = x r with r = 1 / s rounded, then one step q + (x - q s) r.  The step gives the
+// Division by one number for many: q = x r with r = 1 / s rounded, then one step q - (q s - x) r.  The step gives the
 // correctly rounded quotient (P. Markstein, Computation of elementary functions on the IBM RISC System/6000
-// processor, 1990) as long as nothing overflows or vanishes; what is not in a safe range divides.
+// processor, 1990) as long as nothing overflows or vanishes; what is not in a safe range divides.  A remainder of 0 has the
+// sign + , so it is q s - x that is formed: -0 less +0 stays -0, as in a division by a positive s.
 struct Divisor {
     float s, r;
     bool plain;                                     // s in a range where r and the step's products are normal numbers
@@ -71,7 +72,7 @@ __device__ __forceinline__ Divisor divisor(float s) {
 }
 __device__ __forceinline__ float quotient(float x, const Divisor& d) {              // d.plain, |x| up to 2^60
     const float q = __fmul_rn(x, d.r);
-    return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
+    return __fmaf_rn(-__fmaf_rn(q, d.s, -x), d.r, q);
 }
 __device__ __forceinline__ float divide(float x, const Divisor& d) {
     // a quotient so small that the step's remainder vanishes has the code 0 whatever its last bit

@@ -153,3 +153,22 @@ def test_a_computing_warp_that_gives_up_is_reported(lens, H, Hkv, n, fp8):
         assert lib.aa_paged_attend(ctypes.byref(a), stream) == 0
         assert lib.aa_paged_check_status(status.data_ptr(), stream) == 0
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+# ------------------------------------------------------------------------------------------------------- append
+def test_e4m3_codes_of_negative_zeros():
+    """-0 / scale is -0, whose code is 0x80; for scales the kernel multiplies by the reciprocal of and for one it divides by."""
+    scales = torch.tensor([1.0, 0.37, 3e-30])
+    x = torch.zeros(16, 3, 128)
+    x[:, :, ::2] = -0.0
+    x[:, :, 1::4] = torch.tensor([-1e-38, 2.0 ** -40])[None, None].repeat(16, 3, 16) * scales[:, None].clamp(min=1.0)
+    x = x.bfloat16()
+    k = torch.full((1, 3, 16, 128), 1.0, device="cuda").to(torch.float8_e4m3fn)
+    v = k.clone()
+    one = torch.tensor([16], dtype=torch.int32, device="cuda")
+    aa.paged_kv_append(x.cuda(), x.flip(0).cuda(), k, v, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), one,
+                       cu_seqlens=torch.tensor([0, 16], dtype=torch.int32, device="cuda"), k_scale=scales.cuda(), v_scale=scales.cuda())
+    for pool, y in ((k, x), (v, x.flip(0))):
+        want = (y.float() / scales[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        assert (want[:, :, ::2].view(torch.uint8) == 0x80).all()
+        assert torch.equal(pool[0].transpose(0, 1).cpu().view(torch.uint8), want.view(torch.uint8))
