@@ -10,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libanchor_attn_b200.so")
 
 AA_OK = 0
+AA_ERR_CUDA = -10
 AA_BF16 = 0
 AA_E4M3 = 1
 
@@ -206,6 +207,6 @@ def load():
 def error_text(code: int) -> str:
     lib = load()
     msg = lib.aa_strerror(code).decode()
-    if code == -10:
+    if code == AA_ERR_CUDA:
         msg += ": " + lib.aa_last_cuda_error().decode()
     return msg

@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <utility>
+
 #include "page_select.cuh"
 #include "paged_append.cuh"
 #include "paged_attend.cuh"
@@ -301,11 +303,16 @@ int aa_paged_check_status(uint32_t* status, void* stream) {
     if (e != cudaSuccess) return record_cuda_error(e, "cudaMemcpyAsync(status)");
     e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return record_cuda_error(e, "cudaStreamSynchronize");
-    if (!word) return AA_OK;
-    e = cudaMemsetAsync(status, 0, sizeof(word), st);
-    if (e != cudaSuccess) return record_cuda_error(e, "cudaMemsetAsync(status)");
-    if (word & aa::paged::kStatusTimeout) return AA_ERR_DEVICE_TIMEOUT;
-    return word & aa::paged::kStatusBadPage ? AA_ERR_BAD_PAGE : AA_ERR_TOO_LONG;
+    // one kind a call: the bit that is reported is cleared, and no other
+    for (const auto& [bit, code] : {std::pair{aa::paged::kStatusTimeout, AA_ERR_DEVICE_TIMEOUT},
+                                    std::pair{aa::paged::kStatusBadPage, AA_ERR_BAD_PAGE},
+                                    std::pair{aa::paged::kStatusTooLong, AA_ERR_TOO_LONG}}) {
+        if (!(word & bit)) continue;
+        aa::paged::clear_status_kernel<<<1, 1, 0, st>>>(status, bit);
+        e = cudaGetLastError();
+        return e == cudaSuccess ? (int)code : record_cuda_error(e, "launch clear_status");
+    }
+    return AA_OK;
 }
 
 int aa_paged_append(const aa_paged_append_t* a, void* stream) {

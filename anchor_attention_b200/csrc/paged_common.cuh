@@ -17,6 +17,9 @@ constexpr uint32_t kStatusBadPage = 1;   // a page number outside the pool, or a
 constexpr uint32_t kStatusTooLong = 2;   // a sequence longer than its row of the block table, or than the rotary tables
 constexpr uint32_t kStatusTimeout = 4;   // a bounded wait gave up
 
+// Clears bits that the host has read.  Other streams may set others meanwhile.
+__global__ void clear_status_kernel(uint32_t* status, uint32_t bits) { atomicAnd(status, ~bits); }
+
 // An 8-bit code's scale is the largest magnitude times this: the product, not a division, is the definition.
 constexpr float kInv127 = 1.0f / 127.0f;
 

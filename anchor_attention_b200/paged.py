@@ -68,16 +68,24 @@ def _new_status_word(index: int) -> torch.Tensor:
 def check_paged_status(device=None) -> None:
     """Synchronises the current stream and raises if a call since the last check met a page number outside the
     pool, a list entry outside its sequence, or a sequence longer than its row of the block table (or than
-    the rotary tables), or if a bounded wait of the attention kernel gave up."""
+    the rotary tables), or if a bounded wait of the attention kernel gave up.  The message names every kind that was met, and what it
+    names is cleared.  Work of other streams is covered as far as it is done: wait for it first."""
     index = torch.device(device).index if device is not None else None
     index = torch.cuda.current_device() if index is None else index
     word = _status.get(index)
     if word is None:
         return
+    check, met = _lib.load().aa_paged_check_status, {}
     with torch.cuda.device(index):
-        rc = _lib.load().aa_paged_check_status(word.data_ptr(), torch.cuda.current_stream().cuda_stream)
-    if rc != _lib.AA_OK:
-        raise RuntimeError(f"paged cache: {_lib.error_text(rc)}")
+        for _ in range(3):                                   # the kinds there are, one a call
+            rc = check(word.data_ptr(), torch.cuda.current_stream().cuda_stream)
+            if rc == _lib.AA_OK:
+                break
+            met[rc] = _lib.error_text(rc)
+            if rc == _lib.AA_ERR_CUDA:
+                break
+    if met:
+        raise RuntimeError(f"paged cache: {'; '.join(met.values())}")
 
 
 def rotary_tables(inv_freq: torch.Tensor, positions: int) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -373,7 +373,8 @@ int aa_dense_causal_attend(const aa_dense_causal_t *a, void *stream);
  * ones included; 0 marks padding.
  * Device memory that is wrong is not turned into an address: a page number outside the pool is left out (nothing
  * is written, its keys are not attended), a length beyond the table row is cut, and a bit of *status is set (1:
- * page number, 2: length, 4: a bounded wait gave up, its call's results are incomplete).  *status is never cleared by a launch; aa_paged_check_status reads and clears it.
+ * page number, 2: length, 4: a bounded wait gave up, its call's results are incomplete).  *status is never cleared by a
+ * launch; aa_paged_check_status reports and clears it.
  */
 typedef struct aa_paged_cache {
     void   *k_pages, *v_pages;
@@ -390,8 +391,9 @@ typedef struct aa_paged_cache {
     int32_t B;
 } aa_paged_cache_t;
 
-/* Reads the status word (synchronises the stream), clears it: AA_OK, AA_ERR_DEVICE_TIMEOUT, AA_ERR_BAD_PAGE or
- * AA_ERR_TOO_LONG, the first of these that holds. */
+/* Reads the status word (synchronises the stream): AA_OK, AA_ERR_DEVICE_TIMEOUT, AA_ERR_BAD_PAGE or AA_ERR_TOO_LONG, the
+ * first of the errors that holds.  The bit of the error that is returned is cleared, in stream order, and no other: call
+ * again until AA_OK to hear of all.  Calls on other streams are covered as far as they are done. */
 int aa_paged_check_status(uint32_t *status, void *stream);
 
 /*

@@ -172,3 +172,19 @@ def test_e4m3_codes_of_negative_zeros():
         want = (y.float() / scales[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
         assert (want[:, :, ::2].view(torch.uint8) == 0x80).all()
         assert torch.equal(pool[0].transpose(0, 1).cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------------------------------- status
+def test_the_check_reports_every_kind_and_clears_what_it_reports():
+    """A bad page and a length beyond the table in one call: both are named.  The C entry point clears the bit that it reports and
+    no other, so nothing that comes up beside it is lost."""
+    q, k, v, ks, vs, table, lens = _case(2, [40, 33], 16, 4, 2, 1, False)
+    table[0, 1], lens[1] = -7, 1 << 20
+    _run(q, k, v, ks, vs, table, lens)
+    with pytest.raises(RuntimeError, match="outside the pool.*longer than its row"):
+        aa.check_paged_status()
+    aa.check_paged_status()
+    word = torch.tensor([7], dtype=torch.int32, device="cuda")
+    check, stream = _lib.load().aa_paged_check_status, torch.cuda.current_stream().cuda_stream
+    for code, left in ((-11, 3), (-17, 2), (-18, 0), (0, 0)):
+        assert check(word.data_ptr(), stream) == code and word.item() == left
