@@ -6,6 +6,7 @@
 // pass everything on by position.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -88,6 +89,8 @@ bool usable(const at::Tensor& t) {
     for (size_t i = 0; i + 1 < st.size(); ++i) ok = ok && !(st[i] & 7);
     return ok;
 }
+// an expanded view, whose indices share memory: no place to write to
+bool shares_memory(const at::Tensor& t) { return at::has_internal_overlap(t) == at::MemOverlap::Yes; }
 at::Tensor in_place_or_copy(const at::Tensor& t) { return usable(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 bool page_size_ok(int64_t n) { return n >= 16 && n <= 256 && !(n & (n - 1)); }
@@ -243,6 +246,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         a.cache = make_cache(k, v, tensor(args[4], "block_table"), tensor(args[5], "seq_lens"),
                              optional_tensor(args[10], "k_scale"), optional_tensor(args[11], "v_scale"));
         aa_paged_cache_t& c = a.cache;
+        REQUIRE(!shares_memory(k) && !shares_memory(v), "pages of the pools share memory: they cannot be appended to");
         need_rows(key, "key", device);
         need_rows(value, "value", device);
         REQUIRE(key.dim() == 3 && value.sizes() == key.sizes() && key.size(1) == c.Hkv,
@@ -342,6 +346,10 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
             need_rows(out_in, "out", device);
             REQUIRE(out_in.sizes() == query.sizes() && usable(out_in),
                     "out must have the shape of query, contiguous rows and strides and address of 16-byte multiples");
+            REQUIRE(!shares_memory(out_in), "rows of out share memory");
+            // rows are written while others are read
+            REQUIRE(at::get_overlap_status(out_in, query) != at::MemOverlapStatus::Partial,
+                    "out must be query itself or not overlap it");
         }
         c.status = status_word(device);
         const c10::cuda::OptionalCUDAGuard guard(device);

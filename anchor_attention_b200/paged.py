@@ -127,10 +127,10 @@ def paged_decode_attention(query, k_pages, v_pages, block_table, seq_lens, scali
     With ``pages`` (int32 [B, Hkv, width]) and ``page_counts`` (int32 [B, Hkv]), both contiguous, a KV head attends
     only the first ``page_counts`` logical pages of its list, in any order; a page listed twice counts twice.
 
-    Returns the output in the shape of ``query`` (``out``, which may be a strided view or ``query`` itself, if given), and with
-    ``return_lse`` also the natural logarithm of the softmax sums, fp32 of shape ``query.shape[:-1]``.  A row that
-    sees nothing is 0, its logarithm -inf.  Scores, softmax and sums are 32-bit; results depend on the lengths
-    in the batch only through the order of sums."""
+    Returns the output in the shape of ``query`` (``out``, if given: a strided view, or ``query`` itself, but not memory
+    that overlaps it otherwise), and with ``return_lse`` also the natural logarithm of the softmax sums, fp32 of shape
+    ``query.shape[:-1]``.  A row that sees nothing is 0, its logarithm -inf.  Scores, softmax and sums are 32-bit; the
+    other lengths of the batch and the widths of table and lists change results only through the order of sums."""
     return (_binding or _load()).attend(query, k_pages, v_pages, block_table, seq_lens, scaling, k_scale, v_scale, pages,
                                         page_counts, out, return_lse)
 
