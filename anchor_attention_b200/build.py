@@ -2,6 +2,8 @@
 paged cache (_paged_binding.so) with the host compiler against it.
 
     python -m anchor_attention_b200.build [--force] [--verbose]
+
+Without torch (the library alone): python anchor_attention_b200/build.py
 """
 import os
 import subprocess
@@ -49,8 +51,13 @@ def build_library(force=False, verbose=False):
 
 
 def build_binding(verbose=False):
-    """Compile the Python entry points of the paged cache."""
-    import torch
+    """Compile the Python entry points of the paged cache.  Where torch is missing there is nobody to call them: a user of the
+    C interface has the library alone."""
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("torch is not installed: _paged_binding.so is left out, the library is complete\n")
+        return
     torch_dir = os.path.dirname(torch.__file__)
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                os.environ.get("CUDA_HOME", "/usr/local/cuda") + "/include", sysconfig.get_paths()["include"]]

@@ -1,4 +1,5 @@
 """Edge cases of the paged cache's host side that need no GPU."""
+import sys
 import threading
 import types
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 import anchor_attention_b200 as aa
-from anchor_attention_b200 import paged
+from anchor_attention_b200 import build, paged
 
 
 def test_first_calls_of_two_threads_share_a_status_word(monkeypatch):
@@ -64,3 +65,12 @@ def test_pools_whose_pages_share_memory_are_not_appended_to(lib, name):
     args[name] = torch.zeros(1, 2, 16, 128, dtype=torch.bfloat16).expand(8, 2, 16, 128)
     with pytest.raises(AssertionError, match="share memory"):
         aa.paged_kv_append(**args)
+
+
+def test_the_library_builds_where_torch_is_missing(lib, monkeypatch, tmp_path, capsys):
+    """The C interface needs neither torch nor Python: without torch the library is built and the Python entry points are left out."""
+    monkeypatch.setattr(build, "BINDING", str(tmp_path / "_paged_binding.so"))
+    monkeypatch.setitem(sys.modules, "torch", None)                         # importing it raises ImportError
+    assert build.build_library() == build.LIB
+    assert not (tmp_path / "_paged_binding.so").exists()
+    assert "torch" in capsys.readouterr().err
