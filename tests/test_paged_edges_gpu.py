@@ -8,7 +8,7 @@ import torch
 import anchor_attention_b200 as aa
 from anchor_attention_b200 import _lib
 from oracle import paged_oracle as oracle
-from paged_util import make_pool, make_table
+from paged_util import assert_decode, make_pool, make_table
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +188,46 @@ def test_the_check_reports_every_kind_and_clears_what_it_reports():
     check, stream = _lib.load().aa_paged_check_status, torch.cuda.current_stream().cuda_stream
     for code, left in ((-11, 3), (-17, 2), (-18, 0), (0, 0)):
         assert check(word.data_ptr(), stream) == code and word.item() == left
+
+
+# ------------------------------------------------------------------------------------------- tables of any width
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lens,H,Hkv,n", [([5], 8, 2, 1), ([120, 0, 64, 1], 32, 8, 1), ([380], 8, 2, 1), ([250] * 16, 32, 8, 1),
+                                          ([130, 40], 8, 2, 5), ([90], 8, 1, 4), ([4000, 33], 4, 4, 16)])
+def test_attention_with_a_table_wider_than_the_sequences(lens, H, Hkv, n, fp8):
+    """Entries are cut by a rule on the table's width: whole with a narrow table, cut with a wide one.  Both are right."""
+    for width in (None, 8192):
+        q, k, v, ks, vs, table, lens_t = _case(7, lens, 16, H, Hkv, n, fp8, width=width)
+        got, got_lse = _run(q, k, v, ks, vs, table, lens_t)
+        assert_decode(got, got_lse, q, oracle.dequantised(k, ks), oracle.dequantised(v, vs), table[:, :256], lens_t, fp8)
+
+
+@pytest.mark.parametrize("width", [13, 129, 513, 20000])
+def test_selection_with_a_table_wider_than_the_sequences(width):
+    """The blocks of a sequence are chosen by the table's width."""
+    g = torch.Generator().manual_seed(width)
+    lens = [200, 0, 16, 199]
+    table, total = make_table(lens, 16, g, width=width)
+    codes = torch.randint(-127, 128, (total, 2, 128), generator=g, dtype=torch.int8)
+    scales = torch.rand(total, 2, generator=g) / 100
+    q = torch.randn(4, 2, 8, 128, generator=g).bfloat16()
+    lens = torch.tensor(lens, dtype=torch.int32)
+    got = aa.select_pages(*[t.cuda() for t in (q, codes, scales, table, lens)], 6, 16)
+    want = oracle.select(q, codes, scales, table, lens, 6, 16)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+def test_selection_of_the_most_rows():
+    """256 rows a KV head (16 new tokens on a group of 16) are the most that the selection takes; the attention takes more."""
+    g = torch.Generator().manual_seed(1)
+    table, total = make_table([900], 16, g)
+    codes = torch.randint(-127, 128, (total, 1, 128), generator=g, dtype=torch.int8)
+    scales = torch.rand(total, 1, generator=g)
+    lens = torch.tensor([900], dtype=torch.int32)
+    q = torch.randn(1, 16, 16, 128, generator=g).bfloat16()
+    got = aa.select_pages(*[t.cuda() for t in (q, codes, scales, table, lens)], 9, 16)
+    want = oracle.select(q, codes, scales, table, lens, 9, 16)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+    q = torch.randn(1, 16, 17, 128, generator=g).bfloat16()
+    with pytest.raises(RuntimeError, match="too many new tokens"):
+        aa.select_pages(*[t.cuda() for t in (q, codes, scales, table, lens)], 9, 16)
