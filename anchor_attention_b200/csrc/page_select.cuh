@@ -104,8 +104,8 @@ __device__ __forceinline__ int2 block_scan(int2 x, int2& total, int2* s_warp) {
     return before;
 }
 
-// A page's mean key as a matrix operand: lane (g, t) holds the bytes 16 t .. 16 t + 15 and 64 + 16 t .. 64 + 16 t + 15 of
-// pages g and g + 8 of its 16.
+// A lane's share of 16 pages' mean keys: lane (g, t) holds the bytes 16 t .. 16 t + 15 and 64 + 16 t .. 64 + 16 t + 15 of
+// pages g and g + 8.
 struct PageTile {
     uint4 lo[2], hi[2];
     float scale[2];

@@ -363,7 +363,7 @@ int aa_paged_append(const aa_paged_append_t* a, void* stream) {
     else
         tasks = p.per_seq == 1 ? c.B : c.B * ((p.per_seq - 1) / c.page_size + (int64_t)2);
     if (tasks > 0x7FFFFFFF) return AA_ERR_TOO_LARGE;
-    // one token a sequence: a block for every KV head, one for all queries; more tokens: see paged_append.cuh
+    // one token a sequence: a block for every KV head and for every 64 query heads; more tokens: see paged_append.cuh
     const bool single = !a->cu_seqlens && p.per_seq == 1;
     p.kv_heads = single ? 1 : c.page_size < aa::paged::kStagedRows ? aa::paged::kStagedRows / c.page_size : 1;
     p.q_heads = single ? (a->H < 64 ? a->H : 64) : 4 * p.kv_heads;

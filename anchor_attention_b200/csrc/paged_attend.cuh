@@ -10,7 +10,8 @@
 // units of all entries form one line that is cut into as many equal ranges as there are CTAs, whatever the
 // lengths: a batch of unequal sequences and a single long one fill the GPU alike.  Where a cut falls inside an
 // entry, the CTAs on its sides leave (reference, sum, unnormalised row) and paged_join_kernel adds them
-// up in the order of the keys; results depend on the lengths alone, not on timing.  Entries of a few units stay whole.
+// up in the order of the keys.  Entries of a few units stay whole.  Where the cuts fall, and with them the order of the sums,
+// depends on the lengths, the width of the table or lists and the number of SMs, never on timing.
 //
 // Inside a CTA a producer warp walks the units: it looks up their pages and has the TMA copy them (128-byte swizzle)
 // into a ring of stages.  The keys of a unit go to lanes of RW warps, 16 to
@@ -20,14 +21,17 @@
 // the instruction rate was the limit, at 4.9 TB/s.
 // Scores are computed transposed, S^T = K Q^T: the keys fill the 16 rows of the matrix instruction and 8 queries its
 // columns, so a group of 4 wastes half of a tile of 8 instead of three quarters of one of 16; the
-// probabilities then need one 8x8 transpose to become the operand of O^T = V^T P^T.  mma.sync is enough: a
-// tensor-core tile of 128 rows would be filled with padding, and the tensor pipe is busy 16 (bf16) to 38 % of the time
-// (three row tiles).
+// probabilities then need one 8x8 transpose to become the operand of O^T = V^T P^T.  mma.sync is enough for one tile of rows:
+// the tensor pipe is busy 16 % of the time with one tile (bf16), 38 % with three.  With several tiles each of them reads the keys
+// and values from shared memory again.  The same transposed form on tcgen05.mma (keys, then head values, as its 128
+// rows; one reading for all tiles) has not been tried.
 //
-// Measured (B200, whole calls): 32 sequences of up to 32768 tokens, 32/8 heads: bf16 357 to 365 us, 6.6 to 6.8 TB/s; e4m3 188 to
-// 199 us, 6.1 to 6.4 TB/s;
-// one sequence of 131072 tokens 87.5 us, 6.1 TB/s; 16 of up to 4001 tokens 23 us, where the bytes alone
-// take 10; five new tokens for 8 sequences of up to 16001 74 to 79 us, bound by latencies inside a tile.
+// Measured (B200, whole calls, from the fastest to the slowest run on several GPUs): 32 sequences of up to 32768 tokens, 32/8
+// heads: bf16 357 to 369 us, 6.6 to 6.8 TB/s; e4m3 188 to 206 us, 5.9 to 6.4 TB/s;
+// one sequence of 131072 tokens 87.5 to 89.2 us, 6.0 to 6.1 TB/s; 16 of up to 4001 tokens 21 to 23 us, where the bytes alone
+// take 10; five new tokens for 8 sequences of up to 16001 75 to 82 us, bound by latencies inside a tile.
+// The lift of the e4m3 probabilities (see Accuracy) costs 0.5 to 1.5 %.  Registers: 162 to 168, 128 with three row tiles; the e4m3
+// forms of two and four row tiles spill 12 bytes, that of three 68.
 // Without the join kernel (its results then incomplete) calls take 2 us less on the GPU for one short sequence, 3 to 5 us
 // for most, 8 us for the five new tokens.
 //
@@ -55,8 +59,8 @@ constexpr int kMiscBytes = 512;
 constexpr int kSmemBytes = kRingBytes + kCombBytes + kMiscBytes;
 
 // The warps of a CTA (and one more, the producer) and the stages of its ring.  Four computing warps where it can be: two CTAs
-// then leave each thread 162 registers, and a warp that takes two or four tiles of 16 keys a step has enough of its own to
-// hide its latencies.  Measured at 32 sequences of up to 32768 tokens, e4m3, a group of 4: 8 lanes of one tile 196 us, 4 of
+// then have ten warps, three of them on one quarter of the SM, which leaves each thread 168 registers, and a warp that takes two
+// or four tiles of 16 keys a step has enough of its own to hide its latencies.  Measured, each pair in one run, at 32 sequences of up to 32768 tokens, e4m3, a group of 4: 8 lanes of one tile 196 us, 4 of
 // two 188 us; eight sequences of up to 16001 tokens, bf16: 20 rows 85 us with one tile, 74 us with two, 32 rows 99 us with 2 lanes
 // of two tiles, 87 us with one of four, 12 rows 76 us with 4 lanes of one, 66 us with 2 of two; e4m3, 12 rows: 63 and 53 us.
 template <bool FP8, int RW>
@@ -720,7 +724,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     if (r >= p.rows) return;
     auto index = [&](int i) { return ((int64_t)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * tile_rows + rr; };
 
-    // warp w takes parts w, w + 8, ...; the first are on their way while every warp finds the maximum of all
+    // warp w takes parts w, w + 4, ...; the first are on their way while every warp finds the maximum of all
     float4 x[kAhead];
     float2 ml[kAhead];
     auto fetch = [&](int i0) {

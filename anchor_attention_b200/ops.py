@@ -388,7 +388,7 @@ def dense_causal_attention(query, key, value, scaling: float = None, out: Option
     D = 128; row i attends keys 0 .. kv - q + i.  Returns [B,H,q,D] (``out`` may be a strided view,
     e.g. of token-major memory).  The path the reference sends to flash-attn for the tail of a
     prefill and for later chunks (anchor_attn/src/modules/llama/anchor_attention.py:76-88, 101-113).
-    A prefill kernel (128-row tiles): single-token decode should keep using a split-KV library kernel."""
+    A prefill kernel (128-row tiles): one or a few tokens over a paged cache are ``paged_decode_attention``'s work."""
     lib = _lib.load()
     assert query.is_cuda and key.is_cuda and value.is_cuda, "dense_causal_attention takes CUDA tensors (no CPU path)"
     assert query.dtype == torch.bfloat16 and key.dtype == query.dtype and value.dtype == query.dtype

@@ -21,6 +21,9 @@ padding).  What follows a sequence's last page in its row of the table is not re
 All launches are asynchronous on the current stream of the tensors' device.  Nothing is synchronised, so page
 numbers and lengths are checked on the device: a bad one is never used as an address, what it names is left
 out, and ``check_paged_status`` raises for it afterwards.
+
+The functions are for inference: no gradients flow through them.  They are not registered as torch operators, so
+``torch.compile`` breaks its graph at a call (``fullgraph=True`` refuses it); CUDA graphs capture them.
 """
 from __future__ import annotations
 
@@ -102,7 +105,8 @@ def paged_kv_append(key, value, k_pages, v_pages, block_table, seq_lens, cu_seql
     sequence b owns tokens ``cu_seqlens[b]`` .. ``cu_seqlens[b + 1] - 1`` (int32 [B + 1]), or T / B tokens where
     ``cu_seqlens`` is None; they take the positions ``seq_lens[b] - n`` .. ``seq_lens[b] - 1`` and must fall
     on pages no other sequence appends to.  Tokens that would take a negative position (all of a sequence of
-    length 0) and tokens behind ``cu_seqlens[B]`` are padding: nothing of theirs is written.
+    length 0) and tokens behind ``cu_seqlens[B]`` are padding: nothing of theirs is written.  ``cu_seqlens`` must ascend from 0
+    or more to at most T; a range that does not is left out like padding, and not reported.
 
     With ``cos`` and ``sin`` (fp32 [positions, 64], see ``rotary_tables``) keys are rotated (rotate-half) by their
     position, in 32 bits with one rounding at the end.  ``query`` [T, H, 128] is rotated likewise.  With
@@ -125,7 +129,8 @@ def paged_decode_attention(query, k_pages, v_pages, block_table, seq_lens, scali
     all keys the same weight).
 
     With ``pages`` (int32 [B, Hkv, width]) and ``page_counts`` (int32 [B, Hkv]), both contiguous, a KV head attends
-    only the first ``page_counts`` logical pages of its list, in any order; a page listed twice counts twice.
+    only the first ``page_counts`` logical pages of its list, in any order; a page listed twice counts twice.  Tables and lists
+    may name up to 2^30 tokens a row, n * H / Hkv may be up to 65536 (the cache is read once for every 32 of these rows).
 
     Returns the output in the shape of ``query`` (``out``, if given: a strided view, or ``query`` itself, but not memory
     that overlaps it otherwise), and with ``return_lse`` also the natural logarithm of the softmax sums, fp32 of shape
@@ -142,7 +147,7 @@ def select_pages(query, key_codes, key_code_scales, block_table, seq_lens, top_k
     ``paged_kv_append``) scores best against the head's query rows, ``top_k`` in all.  ``query`` as in
     ``paged_decode_attention``, rotated and finite.  A score is the maximum over the rows of the 8-bit dot product
     times both scales; a tie goes to the lower page.  ``keep_last`` must be at least 1: a last page that is not full has
-    no mean yet.
+    no mean yet.  The block table may be up to 40960 pages wide, and n * H / Hkv up to 256; more is refused.
 
     Returns ``(pages int32 [B, Hkv, top_k], counts int32 [B, Hkv])``: logical pages, ascending, -1 behind the
     counts."""

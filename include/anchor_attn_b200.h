@@ -400,7 +400,8 @@ int aa_paged_check_status(uint32_t *status, void *stream);
  * Appends T new tokens: key, value [T, Hkv, 128] bf16 (strides in elements, multiples of 8).  Sequence b owns the
  * tokens cu_seqlens[b] .. cu_seqlens[b+1] - 1 (cu_seqlens int32 [B+1]), or T / B tokens each where
  * cu_seqlens is NULL; they take the positions seq_lens[b] - n .. seq_lens[b] - 1, and what falls on a negative
- * position is padding and is left out, as are tokens behind cu_seqlens[B].  With cos / sin (fp32 [rope_rows, 64],
+ * position is padding and is left out, as are tokens behind cu_seqlens[B] and, unreported, ranges that descend or leave
+ * 0 .. T.  With cos / sin (fp32 [rope_rows, 64],
  * contiguous) keys are rotated with the rotate-half formulation by their position's row, in 32 bits and rounded
  * once; query [T, H, 128] likewise into query_out (NULL: no queries), rotated keys also into key_out (NULL:
  * not wanted).  A sequence must not share a page it appends to.
@@ -461,7 +462,8 @@ int aa_selftest_paged_wait(const aa_paged_attend_t *a, void *stream);
  * query row q [B, Nq, H, 128] has the scale max|q| * (1 / 127) and the codes rint(q / scale); a tie goes to the lower page.
  * out int32 [B, Hkv, top]: logical pages, ascending, -1 behind counts int32 [B, Hkv].  keep_last >= 1 covers a last
  * page that is not full and so has no codes yet; keep_first + keep_last <= top.  Only the table, the lengths and
- * the shape fields of `cache` are read, the pool pointers and strides are not.  One launch.
+ * the shape fields of `cache` are read, the pool pointers and strides are not.  One launch.  table_width up to 40960
+ * (AA_ERR_TOO_LARGE), Nq * H / Hkv up to 256 (AA_ERR_NEW_TOKENS).
  */
 typedef struct aa_page_select {
     aa_paged_cache_t cache;
