@@ -303,8 +303,9 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                         const __grid_constant__ AttendParams p) {
     using S = Shape<FP8, RW>;
     constexpr int kStages = S::kStages, kDepth = S::kDepth;
-    // A state (m, l, o) stands for 2^m l and 2^m o; m is the running maximum less this, so a probability is at most 2^15 in f16.
-    constexpr float kLift = FP8 ? 15.0f : 0.0f;
+    // A state (m, l, o) stands for 2^m l and 2^m o; with e4m3 pages m is the running maximum less this, rounded up: a probability is
+    // at most 2^15 in f16 for scores of any size (from 2^24 on, a difference rounded to nearest could be 16).
+    constexpr float kLift = 15.0f;
     extern __shared__ __align__(1024) uint8_t paged_attend_smem[];
     float* comb = reinterpret_cast<float*>(paged_attend_smem + kRingBytes);
     // the last 512 bytes: barriers, lengths of this range's entries, tile positions of the stages, scratch of the start
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(Shape<FP8, RW>::kThreads, kCtasPerSm)
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                const float m_new = fmaxf(m[x], top - kLift);
+                const float m_new = fmaxf(m[x], FP8 ? __fadd_ru(top, -kLift) : top);
                 const float ref = m_new == -INFINITY ? 0.0f : m_new;       // a row that has seen nothing yet
                 corr[x] = fast_exp2(m[x] - ref);
                 m[x] = m_new;

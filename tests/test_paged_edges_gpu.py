@@ -97,6 +97,33 @@ def test_e4m3_tail_behind_strong_keys():
         assert ((got_lse[b].double().cpu() - lse[0]).abs() <= tol_lse[0]).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("exponent", list(range(16, 36)) + [60, 90, 110])
+def test_scores_so_large_that_one_key_has_all_weight(exponent, fp8):
+    """Scores of 2^exponent and more, where 32 bits hold no small differences: the best key's value comes out, rounded once (the
+    weight's two bf16 parts add 2^-22), and the logarithm is its score (three roundings: scale, product, conversion)."""
+    n, page = 700, 16
+    g = torch.Generator().manual_seed(exponent)
+    level = torch.randint(8, 15, (n,), generator=g).float()
+    best = int(torch.randint(0, n, (1,), generator=g))
+    level[best] = 15.0
+    k = torch.zeros(44, 1, page, 128)
+    k.view(-1, 128)[:n, 0] = level
+    v = (torch.randint(-15, 16, k.shape, generator=g) / 8).float()
+    dtype = torch.float8_e4m3fn if fp8 else torch.bfloat16
+    k, v = k.to(dtype), v.to(dtype)
+    one = torch.ones(1) if fp8 else None
+    q = torch.zeros(1, 1, 4, 128)
+    q[0, 0, :, 0] = torch.tensor([1.0, 1.25, 1.5, 1.75])
+    scaling = 2.0 ** exponent
+    out, lse = _run(q.bfloat16(), k, v, one, one, torch.arange(44, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32),
+                    scaling=scaling)
+    want = v.float().view(-1, 128)[best].double()
+    assert ((out[0, 0].double().cpu() - want).abs() <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all()
+    score = 15.0 * scaling * q[0, 0, :, 0].double()
+    assert ((lse[0, 0].double().cpu() - score).abs() <= 4 * 2.0 ** -24 * score).all()
+
+
 @pytest.mark.parametrize("lens,H,Hkv", [([20000], 8, 1), ([9001, 1, 12000], 8, 2), ([4097] * 40, 4, 4)])
 def test_e4m3_within_the_bounds_of_the_sequences_own_keys(lens, H, Hkv):
     q, k, v, ks, vs, table, lens = _case(3, lens, 64, H, Hkv, 1, True)
