@@ -30,7 +30,9 @@
 // heads: bf16 357 to 369 us, 6.6 to 6.8 TB/s; e4m3 188 to 206 us, 5.9 to 6.4 TB/s;
 // one sequence of 131072 tokens 87.5 to 89.2 us, 6.0 to 6.1 TB/s; 16 of up to 4001 tokens 21 to 23 us, where the bytes alone
 // take 10; five new tokens for 8 sequences of up to 16001 75 to 82 us, bound by latencies inside a tile.
-// The lift of the e4m3 probabilities (see Accuracy) costs 0.5 to 1.5 %.  Registers: 162 to 168, 128 with three row tiles; the e4m3
+// That every warp reports a wait that gave up, and the producer sees its copies land, costs 0.5 to 2 % with e4m3 pages (one token
+// 41.0 and 41.4 us, three 55.5 and 56.5, those 8 sequences), nothing with bf16; the lift of the e4m3 probabilities (see Accuracy)
+// costs nothing.  Registers: 162 to 168, 128 with three row tiles; the e4m3
 // forms of two and four row tiles spill 12 bytes, that of three 68.
 // Without the join kernel (its results then incomplete) calls take 2 us less on the GPU for one short sequence, 3 to 5 us
 // for most, 8 us for the five new tokens.
